@@ -24,6 +24,8 @@
 #include "rows.cuh"
 #include "flow.cuh"
 #include "hift.cuh"
+#include "qknorm.cuh"
+#include "prefix_attn.cuh"
 
 using namespace fcv;
 
@@ -475,6 +477,87 @@ int run_attention(const void* qkv, int dtype, const int32_t* cu, int chunk, cons
     const long kv_rows = cached ? kvs.rows : n_rows;
     FCV_LAUNCH("attn_f32_kernel", attn_f32_kernel, dim3(grid), dim3(kAttnQTile), 0, s, static_cast<const float*>(qkv), src,
                kv, kv_rows, kv_stride, k_col, v_col, t2, n_tiles_dev, chunk, static_cast<float*>(out));
+  }
+  return FCV_OK;
+}
+
+// ------------------------------------------------------------------ query/key norm, shared-prefix attention
+template <typename T, int D>
+int launch_qk_norm(const QkNormArgs& a, bool interleaved, cudaStream_t s) {
+  const long warps = (long)a.N * a.warps_per_row;
+  const long blocks = (warps + 7) / 8;
+  if (blocks > 0x7fffffffL) return fail(FCV_EUNSUPPORTED, "fcv_qk_norm_rope: too many rows (%d)", a.N);
+  if (interleaved)
+    FCV_LAUNCH("qk_norm_rope_kernel", qk_norm_rope_kernel<T, D, true>, dim3((unsigned)blocks), dim3(256), 0, s, a);
+  else
+    FCV_LAUNCH("qk_norm_rope_kernel", qk_norm_rope_kernel<T, D, false>, dim3((unsigned)blocks), dim3(256), 0, s, a);
+  return FCV_OK;
+}
+template <typename T>
+int run_qk_norm(const QkNormArgs& a, int head_dim, bool interleaved, cudaStream_t s) {
+  switch (head_dim) {
+    case 32: return launch_qk_norm<T, 32>(a, interleaved, s);
+    case 64: return launch_qk_norm<T, 64>(a, interleaved, s);
+    case 128: return launch_qk_norm<T, 128>(a, interleaved, s);
+    default: return launch_qk_norm<T, 256>(a, interleaved, s);
+  }
+}
+
+// How a call of the shared-prefix attention is cut: rows of a block and key parts (of the prefix
+// and of a sequence's own keys).
+struct SpPlan {
+  int prefix_rows, own_rows;    // rows of a block
+  int prefix_parts, own_parts;
+  long prefix_blocks;           // row blocks of the prefix
+  size_t bytes;                 // workspace
+};
+SpPlan sp_plan(long N, int B, int H, int Hkv, int D, long P) {
+  SpPlan p{};
+  const long G = H / Hkv;
+  const long rows = N * G, own = (N + B - 1) / B * G;
+  p.prefix_rows = rows <= 16 ? 16 : 64;
+  p.own_rows = own <= 16 ? 16 : 64;
+  p.prefix_blocks = (rows + p.prefix_rows - 1) / p.prefix_rows;
+  // enough blocks for two on every SM, no part under 256 keys
+  const long want = 2L * num_sms();
+  auto parts = [&](long blocks, long most) {
+    return (int)std::max(1L, std::min(most, (want + blocks - 1) / std::max(1L, blocks)));
+  };
+  p.prefix_parts = P > 0 ? parts(p.prefix_blocks * Hkv, std::min(64L, (P + 255) / 256)) : 0;
+  const long own_blocks = (long)B * Hkv * ((own + p.own_rows - 1) / p.own_rows);
+  p.own_parts = parts(own_blocks, 16);
+  const int total = p.prefix_parts + p.own_parts;
+  if (total > 1) p.bytes = (size_t)total * N * H * (D * sizeof(float) + sizeof(float2));
+  return p;
+}
+
+template <typename T, int D, int RP, int RO>
+int launch_sp_pieces(const SpArgs& a, dim3 grid, cudaStream_t s) {
+  constexpr int R = RP > RO ? RP : RO;
+  int smem;
+  if constexpr (sizeof(T) == 2) smem = SpMma<D>::kSmem;
+  else smem = SpF32<D, R / 16>::kSmem;
+  static bool attr[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!attr[dev & 63]) {
+    FCV_CUDA(cudaFuncSetAttribute(sp_pieces_kernel<T, D, RP, RO>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
+    attr[dev & 63] = true;
+  }
+  FCV_LAUNCH("sp_pieces_kernel", sp_pieces_kernel<T, D, RP, RO>, grid, dim3(sizeof(T) == 2 ? 128 : 256), smem, s, a);
+  return FCV_OK;
+}
+template <typename T, int D>
+int run_sp(const SpArgs& a, const SpPlan& p, cudaStream_t s) {
+  const long blocks = (long)a.prefix_items + (long)a.B * a.Hkv * a.own_parts;
+  if (blocks > 0x7fffffffL) return fail(FCV_EUNSUPPORTED, "fcv_shared_prefix_attention: too many blocks");
+  const dim3 grid((unsigned)blocks, (unsigned)a.own_rows);
+  if (p.prefix_rows == 16 && p.own_rows == 16) FCV_TRY((launch_sp_pieces<T, D, 16, 16>(a, grid, s)));
+  else if (p.own_rows == 16) FCV_TRY((launch_sp_pieces<T, D, 64, 16>(a, grid, s)));
+  else FCV_TRY((launch_sp_pieces<T, D, 64, 64>(a, grid, s)));
+  if (a.prefix_parts + a.own_parts > 1) {
+    const long warps = (long)a.N * a.H;
+    FCV_LAUNCH("sp_join_kernel", sp_join_kernel<T, D>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, s, a);
   }
   return FCV_OK;
 }
@@ -949,6 +1032,135 @@ int fcv_attention(const void* qkv, int dtype, const int32_t* cu_seqlens, int B, 
   if (N == 0) return FCV_OK;
   return run_attention(qkv, dtype, cu_seqlens, chunk, tiles, n_tiles, out, N, as_stream(stream), nullptr, sched,
                        sched_ctas);
+}
+
+int fcv_qk_norm_rope(const void* qkv, int dtype, int N, long row_stride, int heads, int kv_heads, int head_dim,
+                     const float* q_weight, const float* k_weight, float eps, const float* rope_cos,
+                     const float* rope_sin, int rope_rows, int rope_half, int interleaved, const int32_t* positions,
+                     void* q_out, long q_stride, void* k_out, long k_stride, void* v_out, long v_stride,
+                     const int32_t* kv_rows, long kv_limit, void* stream) {
+  if (!valid_dtype(dtype)) return fail(FCV_EINVAL, "fcv_qk_norm_rope: bad dtype");
+  if (N < 0 || heads < 1 || kv_heads < 1 || !(eps >= 0.f) || rope_rows < 0 || kv_limit < 0)
+    return fail(FCV_EINVAL, "fcv_qk_norm_rope: bad arguments");
+  if (head_dim != 32 && head_dim != 64 && head_dim != 128 && head_dim != 256)
+    return fail(FCV_EUNSUPPORTED, "fcv_qk_norm_rope: head_dim must be 32, 64, 128 or 256 (got %d)", head_dim);
+  if (rope_half < 8 || rope_half % 8 != 0 || 2 * rope_half > head_dim)
+    return fail(FCV_EUNSUPPORTED, "fcv_qk_norm_rope: the rotated width 2 * %d must be a multiple of 16 of at most "
+                "head_dim", rope_half);
+  if (N == 0) return FCV_OK;
+  if (!qkv || !rope_cos || !rope_sin || !positions || !q_out || !k_out)
+    return fail(FCV_EINVAL, "fcv_qk_norm_rope: null pointer");
+  const long es = (long)dsize(dtype);
+  const uintptr_t at = reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out) |
+                       reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out) |
+                       reinterpret_cast<uintptr_t>(rope_cos) | reinterpret_cast<uintptr_t>(rope_sin) |
+                       reinterpret_cast<uintptr_t>(q_weight) | reinterpret_cast<uintptr_t>(k_weight);
+  if ((at & 15) || ((row_stride * es) & 15) || ((q_stride * es) & 15) || ((k_stride * es) & 15) ||
+      ((v_stride * es) & 15))
+    return fail(FCV_EINVAL, "fcv_qk_norm_rope: rows, weights and tables must be 16-byte aligned");
+  if (!kv_rows && kv_limit < N) return fail(FCV_EINVAL, "fcv_qk_norm_rope: %d rows into %ld", N, kv_limit);
+  QkNormArgs a{};
+  a.qkv = qkv;
+  a.row_stride = row_stride;
+  a.N = N;
+  a.heads = heads;
+  a.kv_heads = kv_heads;
+  a.q_weight = q_weight;
+  a.k_weight = k_weight;
+  a.eps = eps;
+  a.cos = rope_cos;
+  a.sin = rope_sin;
+  a.rope_rows = rope_rows;
+  a.half = rope_half;
+  a.positions = positions;
+  a.q_out = q_out;
+  a.q_stride = q_stride;
+  a.k_out = k_out;
+  a.k_stride = k_stride;
+  a.v_out = v_out;
+  a.v_stride = v_stride;
+  a.kv_rows = kv_rows;
+  a.kv_limit = kv_limit;
+  // a warp per token once there are enough tokens to fill the GPU; fewer tokens share out their heads
+  const int steps = (heads + (v_out ? 2 : 1) * kv_heads + 256 / head_dim - 1) / (256 / head_dim);
+  const long want = 32L * num_sms();
+  a.warps_per_row = (int)std::max(1L, std::min((long)steps, want / N));
+  cudaStream_t s = as_stream(stream);
+  return dtype == FCV_DTYPE_BF16 ? run_qk_norm<bf16>(a, head_dim, interleaved != 0, s)
+                                 : run_qk_norm<float>(a, head_dim, interleaved != 0, s);
+}
+
+size_t fcv_shared_prefix_workspace_bytes(int N, int B, int heads, int kv_heads, int head_dim, int P) {
+  if (N <= 0 || B <= 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || P < 0) return 0;
+  return sp_plan(N, B, heads, kv_heads, head_dim, P).bytes;
+}
+
+int fcv_shared_prefix_attention(const void* q, long q_stride, const void* k, long k_stride, const void* v,
+                                long v_stride, long kv_rows, const void* prefix_k, long prefix_k_stride,
+                                const void* prefix_v, long prefix_v_stride, int P, int dtype,
+                                const int32_t* cu_seqlens, const int32_t* kv_base, const int32_t* kv_lens, int B,
+                                int N, int heads, int kv_heads, int head_dim, int chunk, float scale, void* out,
+                                long out_stride, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!valid_dtype(dtype)) return fail(FCV_EINVAL, "fcv_shared_prefix_attention: bad dtype");
+  if (B < 0 || N < 0 || P < 0 || kv_rows < 0 || chunk < 0 || heads < 1 || kv_heads < 1)
+    return fail(FCV_EINVAL, "fcv_shared_prefix_attention: bad arguments");
+  if (heads % kv_heads != 0)
+    return fail(FCV_EINVAL, "fcv_shared_prefix_attention: %d heads over %d key heads", heads, kv_heads);
+  if (head_dim != 64 && head_dim != 128)
+    return fail(FCV_EUNSUPPORTED, "fcv_shared_prefix_attention: head_dim must be 64 or 128 (got %d)", head_dim);
+  if (N == 0 || B == 0) return FCV_OK;
+  if (!q || !cu_seqlens || !out || (kv_rows > 0 && (!k || !v)) || (P > 0 && (!prefix_k || !prefix_v)) ||
+      (!kv_base != !kv_lens))
+    return fail(FCV_EINVAL, "fcv_shared_prefix_attention: null pointer");
+  const long es = (long)dsize(dtype);
+  const uintptr_t at = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
+                       reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(prefix_k) |
+                       reinterpret_cast<uintptr_t>(prefix_v) | reinterpret_cast<uintptr_t>(out);
+  if ((at & 15) || ((q_stride * es) & 15) || ((k_stride * es) & 15) || ((v_stride * es) & 15) ||
+      ((prefix_k_stride * es) & 15) || ((prefix_v_stride * es) & 15) || ((out_stride * es) & 15))
+    return fail(FCV_EINVAL, "fcv_shared_prefix_attention: rows must be 16-byte aligned");
+  const SpPlan p = sp_plan(N, B, heads, kv_heads, head_dim, P);
+  if (workspace_bytes < p.bytes || (p.bytes && !workspace) || (reinterpret_cast<uintptr_t>(workspace) & 15))
+    return fail(FCV_EINVAL, "fcv_shared_prefix_attention: workspace of %zu bytes, %zu needed", workspace_bytes, p.bytes);
+  if (p.prefix_blocks * kv_heads * p.prefix_parts > 0x7fffffffL)
+    return fail(FCV_EUNSUPPORTED, "fcv_shared_prefix_attention: too many blocks");
+  SpArgs a{};
+  a.q = q;
+  a.q_stride = q_stride;
+  a.k = k;
+  a.v = v;
+  a.k_stride = k_stride;
+  a.v_stride = v_stride;
+  a.kv_rows = kv_rows;
+  a.pk = prefix_k;
+  a.pv = prefix_v;
+  a.pk_stride = prefix_k_stride;
+  a.pv_stride = prefix_v_stride;
+  a.P = P;
+  a.cu = cu_seqlens;
+  a.kv_base = kv_base;
+  a.kv_lens = kv_lens;
+  a.B = B;
+  a.N = N;
+  a.H = heads;
+  a.Hkv = kv_heads;
+  a.G = heads / kv_heads;
+  a.chunk = chunk;
+  a.scale_log2 = scale * kLog2e;
+  a.out = out;
+  a.out_stride = out_stride;
+  a.prefix_parts = p.prefix_parts;
+  a.own_parts = p.own_parts;
+  a.prefix_items = (int)(p.prefix_blocks * kv_heads * p.prefix_parts);
+  const long own = ((long)N + B - 1) / B * a.G;
+  a.own_rows = (int)std::min(1024L, (own + p.own_rows - 1) / p.own_rows);
+  const size_t rows = (size_t)(p.prefix_parts + p.own_parts) * N * heads;
+  a.part_o = static_cast<float*>(workspace);
+  a.part_ml = reinterpret_cast<float2*>(static_cast<float*>(workspace) + rows * head_dim);
+  cudaStream_t s = as_stream(stream);
+  if (dtype == FCV_DTYPE_BF16)
+    return head_dim == 64 ? run_sp<bf16, 64>(a, p, s) : run_sp<bf16, 128>(a, p, s);
+  return head_dim == 64 ? run_sp<float, 64>(a, p, s) : run_sp<float, 128>(a, p, s);
 }
 
 int fcv_attn_tiles(const int32_t* lengths_host, int B, int chunk, int32_t* tiles, int cap) {

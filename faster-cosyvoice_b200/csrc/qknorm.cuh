@@ -1,0 +1,194 @@
+// qknorm.cuh -- per-head RMS norm of queries and keys with the position rotation.
+//
+// For every token n of packed [Q | K | V] rows and every head x (D values) of Q and K:
+//     y = x * rsqrt(mean(x^2) + eps) * w            (w: one D-vector for Q, one for K)
+//     (y_a, y_b) -> (y_a c - y_b s, y_b c + y_a s)   c, s = cos/sin[position[n]][i], i < half
+// over the pairs (2i, 2i + 1) (interleaved) or (i, i + half); values past 2 half only get the
+// norm.  Values V are copied when the keys go to a cache.  Sums and products are float32; each
+// output is rounded once.
+#pragma once
+
+#include "fcv_common.cuh"
+
+namespace fcv {
+
+struct QkNormArgs {
+  const void* qkv;
+  long row_stride;  // elements
+  int N, heads, kv_heads;
+  const float* q_weight;  // null: 1
+  const float* k_weight;
+  float eps;
+  const float* cos;  // (rope_rows, half)
+  const float* sin;
+  int rope_rows, half;
+  const int32_t* positions;
+  void* q_out;
+  long q_stride;
+  void* k_out;
+  long k_stride;
+  void* v_out;  // null: values are not copied
+  long v_stride;
+  const int32_t* kv_rows;  // null: token n's keys go to row n; an entry < 0 stores nothing
+  long kv_limit;           // rows of k_out / v_out
+  int warps_per_row;
+};
+
+template <typename T>
+struct Vec8;
+template <>
+struct Vec8<bf16> {
+  uint4 u;
+  __device__ __forceinline__ void load(const bf16* p) { u = *reinterpret_cast<const uint4*>(p); }
+  __device__ __forceinline__ void store(bf16* p) const { *reinterpret_cast<uint4*>(p) = u; }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    const uint32_t w[4] = {u.x, u.y, u.z, u.w};
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[2 * i] = __uint_as_float(w[i] << 16);
+      x[2 * i + 1] = __uint_as_float(w[i] & 0xffff0000u);
+    }
+  }
+  __device__ __forceinline__ void set(const float (&x)[8]) {
+    u = make_uint4(pack_bf16x2(x[0], x[1]), pack_bf16x2(x[2], x[3]), pack_bf16x2(x[4], x[5]),
+                   pack_bf16x2(x[6], x[7]));
+  }
+};
+template <>
+struct Vec8<float> {
+  float4 a, b;
+  __device__ __forceinline__ void load(const float* p) {
+    a = *reinterpret_cast<const float4*>(p);
+    b = *reinterpret_cast<const float4*>(p + 4);
+  }
+  __device__ __forceinline__ void store(float* p) const {
+    *reinterpret_cast<float4*>(p) = a;
+    *reinterpret_cast<float4*>(p + 4) = b;
+  }
+  __device__ __forceinline__ void get(float (&x)[8]) const {
+    x[0] = a.x, x[1] = a.y, x[2] = a.z, x[3] = a.w;
+    x[4] = b.x, x[5] = b.y, x[6] = b.z, x[7] = b.w;
+  }
+  __device__ __forceinline__ void set(const float (&x)[8]) {
+    a = make_float4(x[0], x[1], x[2], x[3]);
+    b = make_float4(x[4], x[5], x[6], x[7]);
+  }
+};
+
+// A warp takes (a share of) one token's heads, 256 / D heads at a time: D / 8 lanes hold a head,
+// 8 values each, so loads and stores are 16 bytes wide (32 in float32) and the sum of squares is a
+// few shuffles.  The token's cos / sin values stay in registers over its heads.  Two groups of
+// heads are loaded before either is finished.
+template <typename T, int D, bool INTERLEAVED>
+__global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QkNormArgs a) {
+  griddep_wait();
+  griddep_launch();
+  constexpr int L = D / 8;          // lanes of a head
+  constexpr int HPW = 32 / L;       // heads of one step of the warp
+  constexpr int U = 2;              // steps in flight
+  const int lane = threadIdx.x & 31;
+  const long w = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
+  const long n = w / a.warps_per_row;
+  const int part = static_cast<int>(w - n * a.warps_per_row);
+  if (n >= a.N) return;
+  const int pos = a.positions[n];
+  if (pos < 0 || pos >= a.rope_rows) {
+    if (lane == 0) record_error(601);
+    return;
+  }
+  long kv_row = a.kv_rows ? a.kv_rows[n] : n;
+  if (kv_row >= a.kv_limit) {
+    if (lane == 0) record_error(602);
+    kv_row = -1;
+  }
+  const int sub = lane / L, l = lane % L, d0 = 8 * l;
+  const int units = a.heads + (a.v_out ? 2 : 1) * a.kv_heads;
+  const int qk_units = a.heads + a.kv_heads;
+
+  float wq[8], wk[8], cs[8], sn[8];
+#pragma unroll
+  for (int i = 0; i < 8; ++i) wq[i] = wk[i] = 1.f;
+  Vec8<float> t;
+  if (a.q_weight) t.load(a.q_weight + d0), t.get(wq);
+  if (a.k_weight) t.load(a.k_weight + d0), t.get(wk);
+  // rotation of this lane's values: INTERLEAVED uses pairs 4l .. 4l+3 (cs[0..3]); halves use table
+  // entries d0 mod half, the partner values sitting half / 8 lanes away
+  const bool rot = d0 < 2 * a.half;
+  int src = lane;
+  float sign = 0.f;
+  if (rot) {
+    const long row = (long)pos * a.half;
+    if (INTERLEAVED) {
+      const float4 c4 = *reinterpret_cast<const float4*>(a.cos + row + 4 * l);
+      const float4 s4 = *reinterpret_cast<const float4*>(a.sin + row + 4 * l);
+      cs[0] = c4.x, cs[1] = c4.y, cs[2] = c4.z, cs[3] = c4.w;
+      sn[0] = s4.x, sn[1] = s4.y, sn[2] = s4.z, sn[3] = s4.w;
+    } else {
+      const bool low = d0 < a.half;
+      const long i = row + (low ? d0 : d0 - a.half);
+      t.load(a.cos + i), t.get(cs);
+      t.load(a.sin + i), t.get(sn);
+      src = lane + (low ? a.half / 8 : -a.half / 8);
+      sign = low ? -1.f : 1.f;
+    }
+  }
+  const T* row = static_cast<const T*>(a.qkv) + n * a.row_stride;
+  const int step = HPW * a.warps_per_row;
+  for (int base = part * HPW; base < units; base += U * step) {
+    Vec8<T> v[U];
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = base + u * step + sub;
+      if (h < units) v[u].load(row + (long)h * D + d0);
+    }
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h0 = base + u * step;
+      if (h0 >= units) break;  // warp-uniform
+      const int h = h0 + sub;
+      float x[8];
+      if (h < qk_units) {
+        v[u].get(x);
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) x[i] = 0.f;
+      }
+      float ss = 0.f;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
+#pragma unroll
+      for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
+      const float r = rsqrtf(ss * (1.f / D) + a.eps);
+      const bool is_q = h < a.heads;
+#pragma unroll
+      for (int i = 0; i < 8; ++i) x[i] = x[i] * r * (is_q ? wq[i] : wk[i]);
+      if (INTERLEAVED) {
+        if (rot) {
+#pragma unroll
+          for (int i = 0; i < 4; ++i) {
+            const float p = x[2 * i], q = x[2 * i + 1];
+            x[2 * i] = p * cs[i] - q * sn[i];
+            x[2 * i + 1] = q * cs[i] + p * sn[i];
+          }
+        }
+      } else {
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+          const float other = __shfl_sync(0xffffffffu, x[i], src);
+          if (rot) x[i] = x[i] * cs[i] + sign * other * sn[i];
+        }
+      }
+      if (h < qk_units) v[u].set(x);
+      if (is_q) {
+        v[u].store(static_cast<T*>(a.q_out) + n * a.q_stride + (long)h * D + d0);
+      } else if (h < units && kv_row >= 0) {
+        if (h < qk_units)
+          v[u].store(static_cast<T*>(a.k_out) + kv_row * a.k_stride + (long)(h - a.heads) * D + d0);
+        else
+          v[u].store(static_cast<T*>(a.v_out) + kv_row * a.v_stride + (long)(h - qk_units) * D + d0);
+      }
+    }
+  }
+}
+
+}  // namespace fcv

@@ -67,6 +67,9 @@ EXPORTS = (
     "fcv_pack_rows",
     "fcv_hift_workspace_bytes",
     "fcv_hift_forward",
+    "fcv_qk_norm_rope",
+    "fcv_shared_prefix_workspace_bytes",
+    "fcv_shared_prefix_attention",
 )
 
 
@@ -235,6 +238,11 @@ _SIGNATURES = {
     "fcv_pack_rows": (_i, [_vp, _i, _l, _i, _vp, _i, _i, _vp, _i, _vp]),
     "fcv_hift_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(ctypes.c_int)]),
     "fcv_hift_forward": (_i, [ctypes.POINTER(HiftWeights), ctypes.POINTER(HiftBatch), _vp, ctypes.c_size_t, _vp]),
+    "fcv_qk_norm_rope": (_i, [_vp, _i, _i, _l, _i, _i, _i, _vp, _vp, ctypes.c_float, _vp, _vp, _i, _i, _i, _vp, _vp,
+                              _l, _vp, _l, _vp, _l, _vp, _l, _vp]),
+    "fcv_shared_prefix_workspace_bytes": (ctypes.c_size_t, [_i, _i, _i, _i, _i, _i]),
+    "fcv_shared_prefix_attention": (_i, [_vp, _l, _vp, _l, _vp, _l, _l, _vp, _l, _vp, _l, _i, _i, _vp, _vp, _vp, _i,
+                                         _i, _i, _i, _i, _i, ctypes.c_float, _vp, _l, _vp, ctypes.c_size_t, _vp]),
 }
 
 

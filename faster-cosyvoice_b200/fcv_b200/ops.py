@@ -9,6 +9,7 @@ passes device pointers plus the current stream to ``libfcv_b200.so``.
 
 from __future__ import annotations
 
+import contextlib
 import ctypes
 from typing import Sequence
 
@@ -141,6 +142,184 @@ def ragged_attention(qkv: torch.Tensor, cu_seqlens: torch.Tensor, tiles: torch.T
     call("fcv_attention", qkv.data_ptr(), _dt(qkv), cu_seqlens.data_ptr(), cu_seqlens.numel() - 1, N,
          int(max_len), int(chunk), tiles.data_ptr(), int(n_tiles), None if sched is None else sched.data_ptr(),
          int(sched_ctas), out.data_ptr(), _s(qkv))
+    return out
+
+
+def _on(device: torch.device):
+    """Makes ``device`` current for a launch (a no-op when it already is)."""
+    if device.index is None or device.index == torch.cuda.current_device():
+        return contextlib.nullcontext()
+    return torch.cuda.device(device)
+
+
+def _same_device(first: torch.Tensor, **others):
+    """``first`` lives on a CUDA device and so do the given tensors (None: absent)."""
+    if first.device.type != "cuda":
+        raise ValueError("tensors must live on a CUDA device")
+    for name, t in others.items():
+        if t is not None and t.device != first.device:
+            raise ValueError(f"{name} must live on {first.device}")
+
+
+def _int32(name: str, t: torch.Tensor | None, shape: tuple):
+    if t is not None and (t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous()):
+        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape}")
+
+
+def _head_rows(name: str, t: torch.Tensor, heads: int, head_dim: int, dtype: torch.dtype):
+    """(rows, heads, head_dim) with heads packed inside a row; rows may be strided."""
+    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != head_dim or t.dtype != dtype:
+        raise ValueError(f"{name} must be (rows, {heads}, {head_dim}) of {dtype}")
+    if t.shape[0] > 0 and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != head_dim)):
+        raise ValueError(f"the heads of a {name} row must be contiguous")
+
+
+def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """Whether the address ranges of two (row-strided) tensors meet."""
+    if a.numel() == 0 or b.numel() == 0:
+        return False
+    ends = [t.data_ptr() + (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))) * t.element_size()
+            for t in (a, b)]
+    return a.data_ptr() < ends[1] and b.data_ptr() < ends[0]
+
+
+def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: torch.Tensor | None,
+                 rope_cos: torch.Tensor, rope_sin: torch.Tensor, positions: torch.Tensor, heads: int, kv_heads: int,
+                 *, eps: float = 1e-6, interleaved: bool = True, inplace: bool = False,
+                 kv_cache: torch.Tensor | None = None,
+                 kv_rows: torch.Tensor | None = None) -> tuple[torch.Tensor, torch.Tensor]:
+    """RMS norm of every query and key head, then the rotation by position, in one pass.
+
+    ``qkv``: (N, (heads + 2 kv_heads) head_dim) packed [Q | K | V] rows (rows may be strided),
+    head_dim 32, 64, 128 or 256.  Each query and key head becomes ``x * rsqrt(mean(x^2) + eps) *
+    weight`` (float32 ``q_weight`` / ``k_weight`` of head_dim values, None = 1); then its first
+    ``2 * rope_cos.shape[1]`` values are rotated by ``rope_cos/rope_sin[positions[n]]`` (float32
+    tables, int32 positions) over the pairs (2i, 2i + 1) (``interleaved``, the convention of the
+    estimator's tables) or (i, i + half).  Values are not touched.
+
+    Returns ``(q, k)``: (N, heads, head_dim) and (N, kv_heads, head_dim), new tensors or, with
+    ``inplace``, views of ``qkv``, whose query and key columns are rewritten.  With ``kv_cache``
+    (rows, 2 kv_heads head_dim) of [K | V] and int32 ``kv_rows`` (N) the keys and the values go to
+    those cache rows instead and ``(q, kv_cache)`` is returned; a negative row stores nothing (a
+    padding token), and the others must differ from one another.
+
+    A position outside the tables or a row outside the cache is not accessed: the token (its keys
+    and values) stays unwritten and :func:`device_error` reports 601 (602)."""
+    if qkv.dim() != 2 or heads < 1 or kv_heads < 1 or qkv.shape[1] % (heads + 2 * kv_heads):
+        raise ValueError("qkv must be (N, (heads + 2 kv_heads) head_dim)")
+    N, D = qkv.shape[0], qkv.shape[1] // (heads + 2 * kv_heads)
+    _same_device(qkv, q_weight=q_weight, k_weight=k_weight, rope_cos=rope_cos, rope_sin=rope_sin,
+                 positions=positions, kv_cache=kv_cache, kv_rows=kv_rows)
+    dt = _dt(qkv)
+    if N > 0 and qkv.stride(1) != 1:
+        raise ValueError("qkv rows must be contiguous")
+    if N > 1 and qkv.stride(0) < qkv.shape[1]:
+        raise ValueError("qkv rows must not overlap")
+    for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
+        if w is not None and (w.dtype != torch.float32 or w.shape != (D,) or not w.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous float32 tensor of shape ({D},)")
+    if rope_cos.dim() != 2 or rope_cos.shape != rope_sin.shape or not (
+            rope_cos.dtype == rope_sin.dtype == torch.float32) or not (
+            rope_cos.is_contiguous() and rope_sin.is_contiguous()):
+        raise ValueError("rope_cos and rope_sin must be contiguous float32 tables of one shape")
+    _int32("positions", positions, (N,))
+    if (kv_cache is None) != (kv_rows is None):
+        raise ValueError("kv_cache and kv_rows go together")
+    es, H_, K_ = qkv.element_size(), heads * D, kv_heads * D
+    if inplace:
+        q = qkv[:, :H_]
+    else:
+        q = torch.empty(N, H_, dtype=qkv.dtype, device=qkv.device)
+    if kv_cache is not None:
+        _int32("kv_rows", kv_rows, (N,))
+        if kv_cache.dim() != 2 or kv_cache.shape[1] != 2 * K_ or kv_cache.dtype != qkv.dtype or (
+                kv_cache.shape[0] > 0 and kv_cache.stride(1) != 1) or (
+                kv_cache.shape[0] > 1 and kv_cache.stride(0) < 2 * K_):
+            raise ValueError(f"kv_cache must be (rows, {2 * K_}) of {qkv.dtype} with contiguous rows")
+        if _overlap(kv_cache, qkv):
+            raise ValueError("kv_cache must not share memory with qkv")
+        k_ptr, k_stride = kv_cache.data_ptr(), kv_cache.stride(0)
+        v_ptr, rows_ptr, limit = k_ptr + K_ * es, kv_rows.data_ptr(), kv_cache.shape[0]
+        second = kv_cache
+        if limit == 0:  # nothing can be stored; any aligned address stands in
+            k_ptr, v_ptr = qkv.data_ptr(), qkv.data_ptr()
+    else:
+        k = qkv[:, H_:H_ + K_] if inplace else torch.empty(N, K_, dtype=qkv.dtype, device=qkv.device)
+        k_ptr, k_stride, v_ptr, rows_ptr, limit = k.data_ptr(), k.stride(0), None, None, N
+        second = k.unflatten(1, (kv_heads, D))
+    with _on(qkv.device):
+        call("fcv_qk_norm_rope", qkv.data_ptr(), dt, N, qkv.stride(0), heads, kv_heads, D,
+             None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(),
+             float(eps), rope_cos.data_ptr(), rope_sin.data_ptr(), rope_cos.shape[0], rope_cos.shape[1],
+             int(interleaved), positions.data_ptr(), q.data_ptr(), q.stride(0), k_ptr, k_stride, v_ptr, k_stride,
+             rows_ptr, limit, _s(qkv))
+    return q.unflatten(1, (heads, D)), second
+
+
+def shared_prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prefix_k: torch.Tensor,
+                            prefix_v: torch.Tensor, cu_seqlens: torch.Tensor, kv_base: torch.Tensor | None = None,
+                            kv_lens: torch.Tensor | None = None, *, chunk: int = 1, scale: float | None = None,
+                            out: torch.Tensor | None = None) -> torch.Tensor:
+    """Attention of a ragged batch whose sequences share one prefix of keys and values.
+
+    ``q``: (N, heads, head_dim) packed query rows, sequence b at ``cu_seqlens[b] ..
+    cu_seqlens[b+1]`` (int32).  ``prefix_k`` / ``prefix_v``: (P, kv_heads, head_dim), seen by every
+    query; they are read once for the whole batch.  ``k`` / ``v``: (rows, kv_heads, head_dim);
+    sequence b owns rows ``kv_base[b] .. kv_base[b] + kv_lens[b]`` (int32, a cache stretch that ends
+    with the keys of its queries), or, without both, the rows of its queries.  Key head j serves
+    query heads ``j * heads / kv_heads ...``.  head_dim is 64 or 128; rows may be strided (column
+    views of a [Q | K | V] or [K | V] buffer), heads inside a row are packed.
+
+    ``chunk``: 1 is causal, 0 shows every own key, c > 1 is the streaming mask of
+    :func:`ragged_attention` over absolute positions (the prefix occupies positions 0 .. P - 1, the
+    queries are the last positions of their sequence).  ``scale`` defaults to head_dim ** -0.5.
+
+    Returns ``out`` (N, heads, head_dim); a query that sees no key gives zeros, rows of ``out``
+    behind ``cu_seqlens[-1]`` are not written.  Row numbers are checked on the device
+    (:func:`device_error` 611, 612).  The cut of the keys into parts depends on the batch, so a
+    sequence's result may differ in the last bits with its company; equal calls give equal bits."""
+    if q.dim() != 3 or prefix_k.dim() != 3:
+        raise ValueError("q must be (N, heads, head_dim), prefix_k (P, kv_heads, head_dim)")
+    N, H, D = q.shape
+    P, Hkv = prefix_k.shape[0], prefix_k.shape[1]
+    _same_device(q, k=k, v=v, prefix_k=prefix_k, prefix_v=prefix_v, cu_seqlens=cu_seqlens, kv_base=kv_base,
+                 kv_lens=kv_lens, out=out)
+    dt, dtype = _dt(q), q.dtype
+    if Hkv < 1 or H < 1 or H % Hkv:
+        raise ValueError(f"{H} query heads do not share {Hkv} key heads evenly")
+    _head_rows("q", q, H, D, dtype)
+    for name, t in (("k", k), ("v", v), ("prefix_k", prefix_k), ("prefix_v", prefix_v)):
+        _head_rows(name, t, Hkv, D, dtype)
+    if k.shape[0] != v.shape[0] or prefix_v.shape[0] != P:
+        raise ValueError("keys and values must have the same rows")
+    B = cu_seqlens.numel() - 1
+    if B < 0:
+        raise ValueError("cu_seqlens must hold at least one entry")
+    _int32("cu_seqlens", cu_seqlens, (B + 1,))
+    if (kv_base is None) != (kv_lens is None):
+        raise ValueError("kv_base and kv_lens go together")
+    _int32("kv_base", kv_base, (B,))
+    _int32("kv_lens", kv_lens, (B,))
+    if chunk < 0:
+        raise ValueError("chunk must not be negative")
+    if out is None:
+        out = torch.empty(N, H, D, dtype=dtype, device=q.device)
+    else:
+        _head_rows("out", out, H, D, dtype)
+        if out.shape[0] != N or (N > 1 and out.stride(0) < H * D):
+            raise ValueError("out must be (N, heads, head_dim) rows that do not overlap")
+        if any(_overlap(out, t) for t in (q, k, v, prefix_k, prefix_v)):
+            raise ValueError("out must not share memory with the inputs")
+    size = _lib.lib().fcv_shared_prefix_workspace_bytes
+    with _on(q.device):
+        need = size(N, B, H, Hkv, D, P)
+        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
+        call("fcv_shared_prefix_attention", q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(),
+             v.stride(0), k.shape[0], prefix_k.data_ptr(), prefix_k.stride(0), prefix_v.data_ptr(),
+             prefix_v.stride(0), P, dt, cu_seqlens.data_ptr(), None if kv_base is None else kv_base.data_ptr(),
+             None if kv_lens is None else kv_lens.data_ptr(), B, N, H, Hkv, D, int(chunk),
+             D ** -0.5 if scale is None else float(scale), out.data_ptr(), out.stride(0),
+             None if ws is None else ws.data_ptr(), need, _s(q))
     return out
 
 

@@ -408,6 +408,52 @@ int fcv_prompt_rows(const void* prompt, const int32_t* prompt_cu, const int32_t*
 int fcv_pack_rows(const void* src, int src_dtype, long batch_stride, int T, const int32_t* cu, int B,
                   int max_len, void* dst, int dst_dtype, void* stream);
 
+/* ------------------------------------------------------------------ query/key norm and rotation
+ * One pass over packed [Q | K | V] rows (N rows `row_stride` elements apart: `heads` query heads,
+ * then `kv_heads` key and `kv_heads` value heads of `head_dim` values).  Every query and key head is
+ * normalised, y = x * rsqrt(mean(x^2) + eps) * weight (weight: head_dim floats, null = 1), and its
+ * first 2 * rope_half values are rotated by cos / sin [positions[n]][i], i < rope_half (tables of
+ * rope_rows x rope_half floats): pairs (2i, 2i + 1) when `interleaved`, else (i, i + rope_half).
+ * No counterpart in the reference, whose DiT has no query/key norm (modules.py:349-407); the
+ * unnormed partial rotation of its estimator is the epilogue FCV_EPI_BIAS_ROPE_QKV.
+ * Queries go to q_out (N rows), keys to k_out and, when v_out is given, the values unchanged to
+ * v_out; kv_rows (int32, N) names the row of k_out / v_out for every token, a negative entry
+ * stores nothing, rows must differ; null: token n goes to row n.  kv_limit = rows of k_out / v_out.
+ * Outputs may be the inputs' own rows (in place).  A position outside the tables leaves the token
+ * unwritten with device error 601, a row >= kv_limit its keys and values with 602.
+ * head_dim 32, 64, 128 or 256; rope_half a multiple of 8; all rows, weights and tables 16-byte
+ * aligned. */
+int fcv_qk_norm_rope(const void* qkv, int dtype, int N, long row_stride, int heads, int kv_heads, int head_dim,
+                     const float* q_weight, const float* k_weight, float eps, const float* rope_cos,
+                     const float* rope_sin, int rope_rows, int rope_half, int interleaved, const int32_t* positions,
+                     void* q_out, long q_stride, void* k_out, long k_stride, void* v_out, long v_stride,
+                     const int32_t* kv_rows, long kv_limit, void* stream);
+
+/* ------------------------------------------------------------------ shared-prefix attention
+ * Attention of a ragged batch whose sequences share one prefix of P keys and values (streams of one
+ * voice behind the same prompt: under the chunk mask the prompt's keys and values are the same in
+ * every stream).  Sequence b has query rows [cu_seqlens[b], cu_seqlens[b+1]) (nq) and own key rows
+ * [kv_base[b], kv_base[b] + kv_lens[b]) (nk) of k / v; both null: its own keys are the rows of its
+ * queries.  Its queries are the last nq of its nk own positions.  Query i sees the whole prefix and
+ * own key j iff chunk = 0 or floor((P + j) / chunk) <= floor((P + nk - nq + i) / chunk) (chunk 1:
+ * causal; the streaming mask of mask.py:127-158 otherwise).  A query that sees no key gives zeros.
+ *   q, out  (N, heads, head_dim) rows q_stride / out_stride elements apart
+ *   k, v    (kv_rows, kv_heads, head_dim);  prefix_k, prefix_v (P, kv_heads, head_dim)
+ * heads is a multiple of kv_heads (query head h reads key head h / (heads / kv_heads)); head_dim is
+ * 64 or 128; rows 16-byte aligned.  Rows of out outside [cu_seqlens[0], cu_seqlens[B]) are left as
+ * they were.  cu_seqlens that decrease or leave [0, N] give device error 611, own keys outside
+ * [0, kv_rows) 612 (the sequence is computed without own keys).  Values must be finite where some
+ * query of the same sequence sees them; rows behind a sequence's own keys may hold anything.
+ * workspace: fcv_shared_prefix_workspace_bytes() bytes, 16-byte aligned; calls that may overlap
+ * need one each. */
+size_t fcv_shared_prefix_workspace_bytes(int N, int B, int heads, int kv_heads, int head_dim, int P);
+int fcv_shared_prefix_attention(const void* q, long q_stride, const void* k, long k_stride, const void* v,
+                                long v_stride, long kv_rows, const void* prefix_k, long prefix_k_stride,
+                                const void* prefix_v, long prefix_v_stride, int P, int dtype,
+                                const int32_t* cu_seqlens, const int32_t* kv_base, const int32_t* kv_lens, int B,
+                                int N, int heads, int kv_heads, int head_dim, int chunk, float scale, void* out,
+                                long out_stride, void* workspace, size_t workspace_bytes, void* stream);
+
 /* ------------------------------------------------------------------ HiFT vocoder
  * CausalHiFTGenerator (cosyvoice/hifigan/generator.py:578-740) as built by
  * builders.py:38-50, over packed requests.  Replaces the per-request
