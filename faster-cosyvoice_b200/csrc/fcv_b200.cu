@@ -1108,6 +1108,7 @@ int fcv_shared_prefix_attention(const void* q, long q_stride, const void* k, lon
     return fail(FCV_EINVAL, "fcv_shared_prefix_attention: %d heads over %d key heads", heads, kv_heads);
   if (head_dim != 64 && head_dim != 128)
     return fail(FCV_EUNSUPPORTED, "fcv_shared_prefix_attention: head_dim must be 64 or 128 (got %d)", head_dim);
+  if (!(scale > 0.f) || scale > 3.0e38f) return fail(FCV_EINVAL, "fcv_shared_prefix_attention: scale must be positive");
   if (N == 0 || B == 0) return FCV_OK;
   if (!q || !cu_seqlens || !out || (kv_rows > 0 && (!k || !v)) || (P > 0 && (!prefix_k || !prefix_v)) ||
       (!kv_base != !kv_lens))

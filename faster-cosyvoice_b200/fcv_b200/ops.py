@@ -145,33 +145,43 @@ def ragged_attention(qkv: torch.Tensor, cu_seqlens: torch.Tensor, tiles: torch.T
     return out
 
 
-def _on(device: torch.device):
-    """Makes ``device`` current for a launch (a no-op when it already is)."""
-    if device.index is None or device.index == torch.cuda.current_device():
-        return contextlib.nullcontext()
-    return torch.cuda.device(device)
+_NO_SWITCH = contextlib.nullcontext()
 
 
-def _same_device(first: torch.Tensor, **others):
-    """``first`` lives on a CUDA device and so do the given tensors (None: absent)."""
-    if first.device.type != "cuda":
+def _on(device: int):
+    """Makes ``device`` current for a launch (nothing to do when it already is)."""
+    return _NO_SWITCH if device == torch.cuda.current_device() else torch.cuda.device(device)
+
+
+def _raw_stream(device: int) -> int:
+    return torch._C._cuda_getCurrentRawStream(device)
+
+
+def _device_of(first: torch.Tensor, others: tuple) -> int:
+    """Index of the CUDA device on which ``first`` lives; the other tensors (None: absent) must too."""
+    dev = first.get_device()
+    if dev < 0:
         raise ValueError("tensors must live on a CUDA device")
-    for name, t in others.items():
-        if t is not None and t.device != first.device:
-            raise ValueError(f"{name} must live on {first.device}")
+    for t in others:
+        if t is not None and t.get_device() != dev:
+            raise ValueError(f"a tensor lives on {t.device}, not on cuda:{dev}")
+    return dev
 
 
-def _int32(name: str, t: torch.Tensor | None, shape: tuple):
-    if t is not None and (t.dtype != torch.int32 or t.shape != shape or not t.is_contiguous()):
-        raise ValueError(f"{name} must be a contiguous int32 tensor of shape {shape}")
+def _int32(name: str, t: torch.Tensor, n: int):
+    if t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {n} entries")
 
 
-def _head_rows(name: str, t: torch.Tensor, heads: int, head_dim: int, dtype: torch.dtype):
-    """(rows, heads, head_dim) with heads packed inside a row; rows may be strided."""
-    if t.dim() != 3 or t.shape[1] != heads or t.shape[2] != head_dim or t.dtype != dtype:
+def _head_rows(name: str, t: torch.Tensor, heads: int, head_dim: int, dtype: torch.dtype) -> tuple[int, int]:
+    """Rows and row stride of a (rows, heads, head_dim) tensor whose heads are packed inside a row."""
+    shape = t.shape
+    if len(shape) != 3 or shape[1] != heads or shape[2] != head_dim or t.dtype is not dtype:
         raise ValueError(f"{name} must be (rows, {heads}, {head_dim}) of {dtype}")
-    if t.shape[0] > 0 and (t.stride(2) != 1 or (heads > 1 and t.stride(1) != head_dim)):
+    row, head, last = t.stride()
+    if shape[0] > 0 and (last != 1 or (head != head_dim and heads > 1)):
         raise ValueError(f"the heads of a {name} row must be contiguous")
+    return shape[0], row
 
 
 def _overlap(a: torch.Tensor, b: torch.Tensor) -> bool:
@@ -205,55 +215,57 @@ def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: tor
 
     A position outside the tables or a row outside the cache is not accessed: the token (its keys
     and values) stays unwritten and :func:`device_error` reports 601 (602)."""
-    if qkv.dim() != 2 or heads < 1 or kv_heads < 1 or qkv.shape[1] % (heads + 2 * kv_heads):
+    shape = qkv.shape
+    if len(shape) != 2 or heads < 1 or kv_heads < 1 or shape[1] % (heads + 2 * kv_heads):
         raise ValueError("qkv must be (N, (heads + 2 kv_heads) head_dim)")
-    N, D = qkv.shape[0], qkv.shape[1] // (heads + 2 * kv_heads)
-    _same_device(qkv, q_weight=q_weight, k_weight=k_weight, rope_cos=rope_cos, rope_sin=rope_sin,
-                 positions=positions, kv_cache=kv_cache, kv_rows=kv_rows)
+    N, width = shape
+    D = width // (heads + 2 * kv_heads)
+    dev = _device_of(qkv, (q_weight, k_weight, rope_cos, rope_sin, positions, kv_cache, kv_rows))
     dt = _dt(qkv)
-    if N > 0 and qkv.stride(1) != 1:
-        raise ValueError("qkv rows must be contiguous")
-    if N > 1 and qkv.stride(0) < qkv.shape[1]:
-        raise ValueError("qkv rows must not overlap")
+    row, last = qkv.stride()
+    if (N > 0 and last != 1) or (N > 1 and row < width):
+        raise ValueError("qkv rows must be contiguous and must not overlap")
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None and (w.dtype != torch.float32 or w.shape != (D,) or not w.is_contiguous()):
+        if w is not None and (w.dtype is not torch.float32 or w.shape != (D,) or not w.is_contiguous()):
             raise ValueError(f"{name} must be a contiguous float32 tensor of shape ({D},)")
-    if rope_cos.dim() != 2 or rope_cos.shape != rope_sin.shape or not (
-            rope_cos.dtype == rope_sin.dtype == torch.float32) or not (
-            rope_cos.is_contiguous() and rope_sin.is_contiguous()):
+    table = rope_cos.shape
+    if (len(table) != 2 or table != rope_sin.shape or rope_cos.dtype is not torch.float32
+            or rope_sin.dtype is not torch.float32 or not rope_cos.is_contiguous() or not rope_sin.is_contiguous()):
         raise ValueError("rope_cos and rope_sin must be contiguous float32 tables of one shape")
-    _int32("positions", positions, (N,))
+    _int32("positions", positions, N)
     if (kv_cache is None) != (kv_rows is None):
         raise ValueError("kv_cache and kv_rows go together")
-    es, H_, K_ = qkv.element_size(), heads * D, kv_heads * D
+    ptr, es, q_width, k_width = qkv.data_ptr(), qkv.element_size(), heads * D, kv_heads * D
     if inplace:
-        q = qkv[:, :H_]
+        q, q_row = qkv.as_strided((N, heads, D), (row, D, 1)), row
     else:
-        q = torch.empty(N, H_, dtype=qkv.dtype, device=qkv.device)
+        q, q_row = qkv.new_empty((N, heads, D)), q_width
+    v_ptr = rows_ptr = None
     if kv_cache is not None:
-        _int32("kv_rows", kv_rows, (N,))
-        if kv_cache.dim() != 2 or kv_cache.shape[1] != 2 * K_ or kv_cache.dtype != qkv.dtype or (
-                kv_cache.shape[0] > 0 and kv_cache.stride(1) != 1) or (
-                kv_cache.shape[0] > 1 and kv_cache.stride(0) < 2 * K_):
-            raise ValueError(f"kv_cache must be (rows, {2 * K_}) of {qkv.dtype} with contiguous rows")
-        if _overlap(kv_cache, qkv):
+        _int32("kv_rows", kv_rows, N)
+        if kv_cache.dim() != 2 or kv_cache.shape[1] != 2 * k_width or kv_cache.dtype is not qkv.dtype:
+            raise ValueError(f"kv_cache must be (rows, {2 * k_width}) of {qkv.dtype}")
+        limit = kv_cache.shape[0]
+        k_row, last = kv_cache.stride()
+        if (limit > 0 and last != 1) or (limit > 1 and k_row < 2 * k_width):
+            raise ValueError("kv_cache rows must be contiguous and must not overlap")
+        k_ptr = kv_cache.data_ptr() if limit else ptr  # without rows nothing is stored
+        if (N > 0 and limit > 0 and k_ptr < ptr + ((N - 1) * row + width) * es
+                and ptr < k_ptr + ((limit - 1) * k_row + 2 * k_width) * es):
             raise ValueError("kv_cache must not share memory with qkv")
-        k_ptr, k_stride = kv_cache.data_ptr(), kv_cache.stride(0)
-        v_ptr, rows_ptr, limit = k_ptr + K_ * es, kv_rows.data_ptr(), kv_cache.shape[0]
-        second = kv_cache
-        if limit == 0:  # nothing can be stored; any aligned address stands in
-            k_ptr, v_ptr = qkv.data_ptr(), qkv.data_ptr()
+        v_ptr, rows_ptr, second = k_ptr + k_width * es, kv_rows.data_ptr(), kv_cache
+    elif inplace:
+        second = qkv.as_strided((N, kv_heads, D), (row, D, 1), qkv.storage_offset() + q_width)
+        k_ptr, k_row, limit = ptr + q_width * es, row, N
     else:
-        k = qkv[:, H_:H_ + K_] if inplace else torch.empty(N, K_, dtype=qkv.dtype, device=qkv.device)
-        k_ptr, k_stride, v_ptr, rows_ptr, limit = k.data_ptr(), k.stride(0), None, None, N
-        second = k.unflatten(1, (kv_heads, D))
-    with _on(qkv.device):
-        call("fcv_qk_norm_rope", qkv.data_ptr(), dt, N, qkv.stride(0), heads, kv_heads, D,
-             None if q_weight is None else q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(),
-             float(eps), rope_cos.data_ptr(), rope_sin.data_ptr(), rope_cos.shape[0], rope_cos.shape[1],
-             int(interleaved), positions.data_ptr(), q.data_ptr(), q.stride(0), k_ptr, k_stride, v_ptr, k_stride,
-             rows_ptr, limit, _s(qkv))
-    return q.unflatten(1, (heads, D)), second
+        second = qkv.new_empty((N, kv_heads, D))
+        k_ptr, k_row, limit = second.data_ptr(), k_width, N
+    with _on(dev):
+        call("fcv_qk_norm_rope", ptr, dt, N, row, heads, kv_heads, D, None if q_weight is None else
+             q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), eps, rope_cos.data_ptr(),
+             rope_sin.data_ptr(), table[0], table[1], interleaved, positions.data_ptr(), q.data_ptr(), q_row, k_ptr,
+             k_row, v_ptr, k_row, rows_ptr, limit, _raw_stream(dev))
+    return q, second
 
 
 def shared_prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, prefix_k: torch.Tensor,
@@ -280,46 +292,50 @@ def shared_prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, p
     sequence's result may differ in the last bits with its company; equal calls give equal bits."""
     if q.dim() != 3 or prefix_k.dim() != 3:
         raise ValueError("q must be (N, heads, head_dim), prefix_k (P, kv_heads, head_dim)")
+    dev = _device_of(q, (k, v, prefix_k, prefix_v, cu_seqlens, kv_base, kv_lens, out))
     N, H, D = q.shape
-    P, Hkv = prefix_k.shape[0], prefix_k.shape[1]
-    _same_device(q, k=k, v=v, prefix_k=prefix_k, prefix_v=prefix_v, cu_seqlens=cu_seqlens, kv_base=kv_base,
-                 kv_lens=kv_lens, out=out)
+    Hkv = prefix_k.shape[1]
     dt, dtype = _dt(q), q.dtype
     if Hkv < 1 or H < 1 or H % Hkv:
         raise ValueError(f"{H} query heads do not share {Hkv} key heads evenly")
-    _head_rows("q", q, H, D, dtype)
-    for name, t in (("k", k), ("v", v), ("prefix_k", prefix_k), ("prefix_v", prefix_v)):
-        _head_rows(name, t, Hkv, D, dtype)
-    if k.shape[0] != v.shape[0] or prefix_v.shape[0] != P:
+    _, q_row = _head_rows("q", q, H, D, dtype)
+    rows, k_row = _head_rows("k", k, Hkv, D, dtype)
+    v_rows, v_row = _head_rows("v", v, Hkv, D, dtype)
+    P, pk_row = _head_rows("prefix_k", prefix_k, Hkv, D, dtype)
+    pv_rows, pv_row = _head_rows("prefix_v", prefix_v, Hkv, D, dtype)
+    if rows != v_rows or P != pv_rows:
         raise ValueError("keys and values must have the same rows")
     B = cu_seqlens.numel() - 1
     if B < 0:
         raise ValueError("cu_seqlens must hold at least one entry")
-    _int32("cu_seqlens", cu_seqlens, (B + 1,))
-    if (kv_base is None) != (kv_lens is None):
+    _int32("cu_seqlens", cu_seqlens, B + 1)
+    base_ptr = lens_ptr = None
+    if kv_base is not None and kv_lens is not None:
+        _int32("kv_base", kv_base, B)
+        _int32("kv_lens", kv_lens, B)
+        base_ptr, lens_ptr = kv_base.data_ptr(), kv_lens.data_ptr()
+    elif kv_base is not None or kv_lens is not None:
         raise ValueError("kv_base and kv_lens go together")
-    _int32("kv_base", kv_base, (B,))
-    _int32("kv_lens", kv_lens, (B,))
     if chunk < 0:
         raise ValueError("chunk must not be negative")
+    if scale is None:
+        scale = D ** -0.5
     if out is None:
-        out = torch.empty(N, H, D, dtype=dtype, device=q.device)
+        out, out_row = q.new_empty((N, H, D)), H * D
     else:
-        _head_rows("out", out, H, D, dtype)
-        if out.shape[0] != N or (N > 1 and out.stride(0) < H * D):
+        out_rows, out_row = _head_rows("out", out, H, D, dtype)
+        if out_rows != N or (N > 1 and out_row < H * D):
             raise ValueError("out must be (N, heads, head_dim) rows that do not overlap")
         if any(_overlap(out, t) for t in (q, k, v, prefix_k, prefix_v)):
             raise ValueError("out must not share memory with the inputs")
-    size = _lib.lib().fcv_shared_prefix_workspace_bytes
-    with _on(q.device):
-        need = size(N, B, H, Hkv, D, P)
-        ws = torch.empty(need, dtype=torch.uint8, device=q.device) if need else None
-        call("fcv_shared_prefix_attention", q.data_ptr(), q.stride(0), k.data_ptr(), k.stride(0), v.data_ptr(),
-             v.stride(0), k.shape[0], prefix_k.data_ptr(), prefix_k.stride(0), prefix_v.data_ptr(),
-             prefix_v.stride(0), P, dt, cu_seqlens.data_ptr(), None if kv_base is None else kv_base.data_ptr(),
-             None if kv_lens is None else kv_lens.data_ptr(), B, N, H, Hkv, D, int(chunk),
-             D ** -0.5 if scale is None else float(scale), out.data_ptr(), out.stride(0),
-             None if ws is None else ws.data_ptr(), need, _s(q))
+    with _on(dev):
+        need = _lib.lib().fcv_shared_prefix_workspace_bytes(N, B, H, Hkv, D, P)
+        # a workspace of this call alone, from the allocator that knows streams and graph captures
+        ws = q.new_empty(need, dtype=torch.uint8) if need else None
+        call("fcv_shared_prefix_attention", q.data_ptr(), q_row, k.data_ptr(), k_row, v.data_ptr(), v_row, rows,
+             prefix_k.data_ptr(), pk_row, prefix_v.data_ptr(), pv_row, P, dt, cu_seqlens.data_ptr(), base_ptr,
+             lens_ptr, B, N, H, Hkv, D, chunk, scale, out.data_ptr(), out_row,
+             None if ws is None else ws.data_ptr(), need, _raw_stream(dev))
     return out
 
 

@@ -440,7 +440,7 @@ int fcv_qk_norm_rope(const void* qkv, int dtype, int N, long row_stride, int hea
  *   q, out  (N, heads, head_dim) rows q_stride / out_stride elements apart
  *   k, v    (kv_rows, kv_heads, head_dim);  prefix_k, prefix_v (P, kv_heads, head_dim)
  * heads is a multiple of kv_heads (query head h reads key head h / (heads / kv_heads)); head_dim is
- * 64 or 128; rows 16-byte aligned.  Rows of out outside [cu_seqlens[0], cu_seqlens[B]) are left as
+ * 64 or 128; scale is positive; rows 16-byte aligned.  Rows of out outside [cu_seqlens[0], cu_seqlens[B]) are left as
  * they were.  cu_seqlens that decrease or leave [0, N] give device error 611, own keys outside
  * [0, kv_rows) 612 (the sequence is computed without own keys).  Values must be finite where some
  * query of the same sequence sees them; rows behind a sequence's own keys may hold anything.

@@ -57,7 +57,8 @@ def test_norm_refuses(lib, bad, status):
     (dict(head_dim=32), -2), (dict(head_dim=256), -2), (dict(q=None), -1), (dict(k=None), -1), (dict(pv=None), -1),
     (dict(cu=None), -1), (dict(out=None), -1), (dict(base=None), -1), (dict(lens=None), -1), (dict(q=A + 2), -1),
     (dict(out=A + 8), -1), (dict(qs=1025), -1), (dict(ks=1025), -1), (dict(pvs=1025), -1), (dict(os=1025), -1),
-    (dict(ws_bytes=16), -1), (dict(ws=None), -1), (dict(ws=A + 4), -1),
+    (dict(ws_bytes=16), -1), (dict(scale=0.0), -1), (dict(scale=-0.1), -1),
+    (dict(scale=float("nan")), -1), (dict(scale=float("inf")), -1), (dict(ws=None), -1), (dict(ws=A + 4), -1),
 ])
 def test_attention_refuses(lib, bad, status):
     assert attend(lib, **bad) == status
