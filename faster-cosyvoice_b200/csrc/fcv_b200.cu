@@ -26,6 +26,7 @@
 #include "hift.cuh"
 #include "qknorm.cuh"
 #include "prefix_attn.cuh"
+#include "prefix_fa.cuh"
 
 using namespace fcv;
 
@@ -503,32 +504,108 @@ int run_qk_norm(const QkNormArgs& a, int head_dim, bool interleaved, cudaStream_
   }
 }
 
-// How a call of the shared-prefix attention is cut: rows of a block and key parts (of the prefix
-// and of a sequence's own keys).
+// How a call of the shared-prefix attention is cut.  Whole items (prefix_fa.cuh) compute a run of
+// one sequence's tokens in one go; otherwise the keys are cut into parts: of the prefix, over
+// stacked rows of the whole batch, and of each sequence's own keys.
 struct SpPlan {
-  int prefix_rows, own_rows;    // rows of a block
+  bool whole;                   // whole items on the tensor cores
+  bool fa_prefix;               // parts of the prefix on the tensor cores
+  int prefix_rows, own_rows;    // rows of a block of sp_pieces_kernel
   int prefix_parts, own_parts;
   long prefix_blocks;           // row blocks of the prefix
+  long list_cap;                // entries of the list of whole items
   size_t bytes;                 // workspace
 };
-SpPlan sp_plan(long N, int B, int H, int Hkv, int D, long P) {
+SpPlan sp_plan(long N, int B, int H, int Hkv, int D, long P, bool bf) {
   SpPlan p{};
   const long G = H / Hkv;
   const long rows = N * G, own = (N + B - 1) / B * G;
+  const long tile = G <= 128 ? 128 / G : 1, block = (D == 64 ? 3 : 2) * tile;  // tokens
+  const long sms = num_sms();
+  p.whole = bf && G <= 128 && own >= 64 && std::max((long)std::min((long)B, N), (N + block - 1) / block) * Hkv >= sms / 2;
+  if (p.whole) {
+    p.list_cap = N / block + B;
+    p.bytes = 16 + (size_t)p.list_cap * sizeof(int2);
+    return p;
+  }
   p.prefix_rows = rows <= 16 ? 16 : 64;
   p.own_rows = own <= 16 ? 16 : 64;
-  p.prefix_blocks = (rows + p.prefix_rows - 1) / p.prefix_rows;
-  // enough blocks for two on every SM, no part under 256 keys
-  const long want = 2L * num_sms();
-  auto parts = [&](long blocks, long most) {
+  p.fa_prefix = bf && G <= 128 && rows >= 128 && P >= 512;
+  p.prefix_blocks = p.fa_prefix ? (N + block - 1) / block : (rows + p.prefix_rows - 1) / p.prefix_rows;
+  // enough blocks for two on every SM (one for the tensor-core kernel), no part under 256 keys
+  auto parts = [&](long want, long blocks, long most) {
     return (int)std::max(1L, std::min(most, (want + blocks - 1) / std::max(1L, blocks)));
   };
-  p.prefix_parts = P > 0 ? parts(p.prefix_blocks * Hkv, std::min(64L, (P + 255) / 256)) : 0;
+  p.prefix_parts = P > 0 ? parts(p.fa_prefix ? sms : 2 * sms, p.prefix_blocks * Hkv, std::min(64L, (P + 255) / 256)) : 0;
   const long own_blocks = (long)B * Hkv * ((own + p.own_rows - 1) / p.own_rows);
-  p.own_parts = parts(own_blocks, 16);
+  p.own_parts = parts(2 * sms, own_blocks, 16);
   const int total = p.prefix_parts + p.own_parts;
   if (total > 1) p.bytes = (size_t)total * N * H * (D * sizeof(float) + sizeof(float2));
   return p;
+}
+
+// 3-D tensor of `d2` x `d1` x `d0` bf16 values, box b2 x b1 x 64, 128-byte swizzle, zero fill.
+int make_tmap_3d(CUtensorMap* m, const void* ptr, long d0, long d1, long d2, long ld1, long ld2, int b1, int b2) {
+  PFN_encodeTiled_t enc = encode_fn();
+  if (!enc) return fail(FCV_ECUDA, "cuTensorMapEncodeTiled unavailable");
+  cuuint64_t gdim[3] = {(cuuint64_t)d0, (cuuint64_t)d1, (cuuint64_t)d2};
+  cuuint64_t gstride[2] = {(cuuint64_t)(ld1 * 2), (cuuint64_t)(ld2 * 2)};
+  cuuint32_t box[3] = {64, (cuuint32_t)b1, (cuuint32_t)b2};
+  cuuint32_t estr[3] = {1, 1, 1};
+  CUresult r = enc(m, CU_TENSOR_MAP_DATA_TYPE_BFLOAT16, 3, const_cast<void*>(ptr), gdim, gstride, box, estr,
+                   CU_TENSOR_MAP_INTERLEAVE_NONE, CU_TENSOR_MAP_SWIZZLE_128B, CU_TENSOR_MAP_L2_PROMOTION_L2_256B,
+                   CU_TENSOR_MAP_FLOAT_OOB_FILL_NONE);
+  if (r != CUDA_SUCCESS) return fail(FCV_ECUDA, "cuTensorMapEncodeTiled failed (%d)", (int)r);
+  return FCV_OK;
+}
+
+// Tensor-core kernel: whole items (list given) or the prefix parts.
+template <int D>
+int launch_sp_fa(const SpArgs& a, const SpPlan& p, int2* list, int* count, cudaStream_t s) {
+  using C = SpFa<D>;
+  SfArgs f{};
+  f.a = a;
+  f.tile_tokens = 128 / a.G;
+  const int block = C::T * f.tile_tokens;
+  const long cols = (long)a.Hkv * D;
+  CUtensorMap tq, tpk, tpv, tk, tv, tv8, tv1;
+  FCV_TRY(make_tmap_3d(&tq, a.q, D, a.H, a.N, D, a.q_stride, a.G, f.tile_tokens));
+  // an absent tensor is stood in for by one query row that nothing reads unmasked
+  const void* pk = a.P > 0 ? a.pk : a.q;
+  const void* pv = a.P > 0 ? a.pv : a.q;
+  FCV_TRY(make_tmap_bf16(&tpk, pk, a.P > 0 ? a.P : 1, cols, a.P > 0 ? a.pk_stride : cols, kSfKeys));
+  FCV_TRY(make_tmap_bf16(&tpv, pv, a.P > 0 ? a.P : 1, cols, a.P > 0 ? a.pv_stride : cols, kSfKeys));
+  const bool own = list && a.kv_rows > 0;
+  const void* k = own ? a.k : a.q;
+  const void* v = own ? a.v : a.q;
+  const long rows = own ? a.kv_rows : 1, ks = own ? a.k_stride : cols, vs = own ? a.v_stride : cols;
+  FCV_TRY(make_tmap_bf16(&tk, k, rows, cols, ks, kSfKeys));
+  FCV_TRY(make_tmap_bf16(&tv, v, rows, cols, vs, kSfKeys));
+  FCV_TRY(make_tmap_bf16(&tv8, v, rows, cols, vs, 8));
+  FCV_TRY(make_tmap_bf16(&tv1, v, rows, cols, vs, 1));
+  f.none_row = (int)rows;
+  long items;
+  if (list) {
+    f.list = list;
+    f.count = count;
+    f.list_cap = (int)p.list_cap;
+    items = p.list_cap * a.Hkv;
+    FCV_LAUNCH("sp_list_kernel", sp_list_kernel, dim3(1), dim3(1024), 0, s, a, block, list, f.list_cap, count);
+  } else {
+    items = p.prefix_blocks * a.Hkv * p.prefix_parts;
+    f.prefix_items = (int)items;
+  }
+  static bool attr[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!attr[dev & 63]) {
+    FCV_CUDA(cudaFuncSetAttribute(sp_fa_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, sf_smem_bytes<D>()));
+    attr[dev & 63] = true;
+  }
+  const int grid = (int)std::min(items, (long)num_sms());
+  FCV_LAUNCH("sp_fa_kernel", sp_fa_kernel<D>, dim3(grid), dim3(C::THREADS), sf_smem_bytes<D>(), s, tq, tpk, tpv, tk,
+             tv, tv8, tv1, f);
+  return FCV_OK;
 }
 
 template <typename T, int D, int RP, int RO>
@@ -549,6 +626,7 @@ int launch_sp_pieces(const SpArgs& a, dim3 grid, cudaStream_t s) {
 }
 template <typename T, int D>
 int run_sp(const SpArgs& a, const SpPlan& p, cudaStream_t s) {
+  if (p.fa_prefix) FCV_TRY(launch_sp_fa<D>(a, p, nullptr, nullptr, s));
   const long blocks = (long)a.prefix_items + (long)a.B * a.Hkv * a.own_parts;
   if (blocks > 0x7fffffffL) return fail(FCV_EUNSUPPORTED, "fcv_shared_prefix_attention: too many blocks");
   const dim3 grid((unsigned)blocks, (unsigned)a.own_rows);
@@ -1090,9 +1168,9 @@ int fcv_qk_norm_rope(const void* qkv, int dtype, int N, long row_stride, int hea
                                  : run_qk_norm<float>(a, head_dim, interleaved != 0, s);
 }
 
-size_t fcv_shared_prefix_workspace_bytes(int N, int B, int heads, int kv_heads, int head_dim, int P) {
-  if (N <= 0 || B <= 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || P < 0) return 0;
-  return sp_plan(N, B, heads, kv_heads, head_dim, P).bytes;
+size_t fcv_shared_prefix_workspace_bytes(int N, int B, int heads, int kv_heads, int head_dim, int P, int dtype) {
+  if (!valid_dtype(dtype) || N <= 0 || B <= 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || P < 0) return 0;
+  return sp_plan(N, B, heads, kv_heads, head_dim, P, dtype == FCV_DTYPE_BF16).bytes;
 }
 
 int fcv_shared_prefix_attention(const void* q, long q_stride, const void* k, long k_stride, const void* v,
@@ -1120,7 +1198,9 @@ int fcv_shared_prefix_attention(const void* q, long q_stride, const void* k, lon
   if ((at & 15) || ((q_stride * es) & 15) || ((k_stride * es) & 15) || ((v_stride * es) & 15) ||
       ((prefix_k_stride * es) & 15) || ((prefix_v_stride * es) & 15) || ((out_stride * es) & 15))
     return fail(FCV_EINVAL, "fcv_shared_prefix_attention: rows must be 16-byte aligned");
-  const SpPlan p = sp_plan(N, B, heads, kv_heads, head_dim, P);
+  if (P > 0x7fffff00 || kv_rows > 0x7fffff00L)  // row numbers of a tile past the last row stay 32-bit
+    return fail(FCV_EUNSUPPORTED, "fcv_shared_prefix_attention: too many key rows");
+  const SpPlan p = sp_plan(N, B, heads, kv_heads, head_dim, P, dtype == FCV_DTYPE_BF16);
   if (workspace_bytes < p.bytes || (p.bytes && !workspace) || (reinterpret_cast<uintptr_t>(workspace) & 15))
     return fail(FCV_EINVAL, "fcv_shared_prefix_attention: workspace of %zu bytes, %zu needed", workspace_bytes, p.bytes);
   if (p.prefix_blocks * kv_heads * p.prefix_parts > 0x7fffffffL)
@@ -1152,13 +1232,18 @@ int fcv_shared_prefix_attention(const void* q, long q_stride, const void* k, lon
   a.out_stride = out_stride;
   a.prefix_parts = p.prefix_parts;
   a.own_parts = p.own_parts;
-  a.prefix_items = (int)(p.prefix_blocks * kv_heads * p.prefix_parts);
+  a.prefix_items = p.fa_prefix ? 0 : (int)(p.prefix_blocks * kv_heads * p.prefix_parts);
+  cudaStream_t s = as_stream(stream);
+  if (p.whole) {
+    int* count = static_cast<int*>(workspace);
+    int2* list = reinterpret_cast<int2*>(count + 4);
+    return head_dim == 64 ? launch_sp_fa<64>(a, p, list, count, s) : launch_sp_fa<128>(a, p, list, count, s);
+  }
   const long own = ((long)N + B - 1) / B * a.G;
   a.own_rows = (int)std::min(1024L, (own + p.own_rows - 1) / p.own_rows);
   const size_t rows = (size_t)(p.prefix_parts + p.own_parts) * N * heads;
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(static_cast<float*>(workspace) + rows * head_dim);
-  cudaStream_t s = as_stream(stream);
   if (dtype == FCV_DTYPE_BF16)
     return head_dim == 64 ? run_sp<bf16, 64>(a, p, s) : run_sp<bf16, 128>(a, p, s);
   return head_dim == 64 ? run_sp<float, 64>(a, p, s) : run_sp<float, 128>(a, p, s);

@@ -73,12 +73,13 @@ def test_empty_calls_return_before_any_launch(lib):
 
 def test_workspace_is_sized_on_the_host(lib):
     size = lib.fcv_shared_prefix_workspace_bytes
-    assert size(0, 4, 16, 16, 64, 100) == 0
-    assert size(4, 0, 16, 16, 64, 100) == 0
-    assert size(4, 4, 16, 3, 64, 100) == 0
-    assert size(4, 4, 16, 16, 64, -1) == 0
+    assert size(0, 4, 16, 16, 64, 100, 1) == 0
+    assert size(4, 0, 16, 16, 64, 100, 1) == 0
+    assert size(4, 4, 16, 3, 64, 100, 1) == 0
+    assert size(4, 4, 16, 16, 64, -1, 1) == 0
     # at least one part of the prefix and one of the own keys: output, maximum and sum of every head
-    assert size(64, 64, 32, 8, 128, 4096) >= 2 * 64 * 32 * (128 * 4 + 8)
+    assert size(4, 4, 16, 16, 64, 100, 5) == 0
+    assert size(64, 64, 32, 8, 128, 4096, 0) >= 2 * 64 * 32 * (128 * 4 + 8)
 
 
 def test_cpu_tensors_are_refused():
