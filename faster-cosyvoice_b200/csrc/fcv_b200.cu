@@ -9,6 +9,7 @@
 
 #include <algorithm>
 #include <atomic>
+#include <cmath>
 #include <cstdarg>
 #include <cstdio>
 #include <cstdlib>
@@ -27,6 +28,7 @@
 #include "qknorm.cuh"
 #include "prefix_attn.cuh"
 #include "prefix_fa.cuh"
+#include "prefix_stream.cuh"
 
 using namespace fcv;
 
@@ -504,43 +506,152 @@ int run_qk_norm(const QkNormArgs& a, int head_dim, bool interleaved, cudaStream_
   }
 }
 
-// How a call of the shared-prefix attention is cut.  Whole items (prefix_fa.cuh) compute a run of
-// one sequence's tokens in one go; otherwise the keys are cut into parts: of the prefix, over
+// How a call of the shared-prefix attention is cut.  Whole: a block computes a run of one
+// sequence's tokens against the prefix and its own keys; on the tensor-core kernel (prefix_fa.cuh) or,
+// for few rows, in sp_pieces_kernel.  Otherwise the keys are cut into parts: of the prefix, over
 // stacked rows of the whole batch, and of each sequence's own keys.
 struct SpPlan {
-  bool whole;                   // whole items on the tensor cores
-  bool fa_prefix;               // parts of the prefix on the tensor cores
+  bool fa_whole;                // whole, on the tensor-core kernel
+  bool whole;                   // whole, in sp_pieces_kernel
+  bool fa_prefix;               // parts of the prefix on the tensor-core kernel
   int prefix_rows, own_rows;    // rows of a block of sp_pieces_kernel
   int prefix_parts, own_parts;
   long prefix_blocks;           // row blocks of the prefix
+  int fa_ctas;                  // blocks of the tensor-core kernel
+  int cuts;                     // stretches (blocks) of sp_stream_kernel, 0: own keys in sp_pieces_kernel
   long list_cap;                // entries of the list of whole items
-  size_t bytes;                 // workspace
+  size_t part_bytes, cut_bytes; // workspace: parts of rows, boundary slots
+  size_t bytes;
+  SpSplit split;
 };
-SpPlan sp_plan(long N, int B, int H, int Hkv, int D, long P, bool bf) {
+// The estimates below choose between the ways of cutting.  They are fits, in microseconds on a B200, to
+// 356 shapes (1 to 128 sequences of 1 to 200 queries, prefixes of 200 to 8000 keys, 60 to 1200 own keys,
+// heads 16/16 and 14/2 of 64, 32/8 and 8/1 of 128) timed each way; the way that they choose is on
+// average 2 % slower than the best of the three.  Examples, tensor-core whole / whole / parts: one query
+// of each of 4 streams behind 200 keys (16/16 heads) 13.4 / 7.4 / 15.7; behind 8000 keys 112 / 60 / 29;
+// 32 sequences of about 170 queries behind 2000 keys (32/8 heads) 256 / 688 / 396.
+// The own keys' lengths are on the device: a cache is taken to be half full.
+SpPlan sp_plan(long N, int B, int H, int Hkv, int D, long P, bool bf, long kv_rows, bool packed) {
   SpPlan p{};
-  const long G = H / Hkv;
-  const long rows = N * G, own = (N + B - 1) / B * G;
+  const long G = H / Hkv, q_len = (N + B - 1) / B;
+  const long rows = N * G, own = q_len * G;  // stacked rows, and of a sequence
   const long tile = G <= 128 ? 128 / G : 1, block = (D == 64 ? 3 : 2) * tile;  // tokens
   const long sms = num_sms();
-  p.whole = bf && G <= 128 && own >= 64 && std::max((long)std::min((long)B, N), (N + block - 1) / block) * Hkv >= sms / 2;
-  if (p.whole) {
+  const long tiles = (P + kSpKeys - 1) / kSpKeys;
+  const long own_len = packed ? (q_len + 1) / 2 : std::min(kv_rows / B, 4096L) / 2;
+  const long own_tiles = std::max(1L, (own_len + kSpKeys - 1) / kSpKeys);
+  const bool tensor = bf && G <= 128;
+  p.prefix_rows = rows <= 16 ? 16 : 64;
+  p.own_rows = own <= 16 ? 16 : 64;
+  const bool stream = tensor && G <= 16 && own <= 16;
+  const int d = D == 64 ? 0 : 1, r = p.own_rows == 16 ? 0 : 1;
+  const double all = (double)(tiles + own_tiles), own_blocks = (double)B * Hkv * ((own + p.own_rows - 1) / p.own_rows);
+  const double load = own_blocks / sms;  // blocks of sp_pieces_kernel on an SM
+  // a tile of one block alone on an SM, and among others
+  static const double kAlone[2][2] = {{0.43, 0.73}, {0.74, 1.2}}, kAmong[2][2] = {{0.26, 0.52}, {0.57, 1.12}};
+  // a tile step of a tensor-core item by its query tiles in use; in full (prefix parts)
+  static const double kStep[2][3] = {{0.78, 1.0, 1.25}, {0.86, 1.1, 1.1}}, kFull[2] = {1.25, 1.1};
+  double fa_us = 1e30, whole_us, parts_us = 1e30;
+  if (tensor) {
+    const long used = std::min((long)(D == 64 ? 3 : 2), (q_len + tile - 1) / tile);
+    const double items = (double)std::min((long)B, N) * ((q_len + block - 1) / block) * Hkv;
+    const double waves = items <= sms ? 1.0 : items / sms + 0.3;
+    fa_us = 10.5 + waves * (all * kStep[d][used - 1] + 1.5);
+    whole_us = 5.5 + 2 * d + (load <= 1 ? all * kAlone[d][r]
+                                        : std::max(all * kAlone[d][r], (load + 0.5) * all * kAmong[d][r]) + 0.3 * load);
+    const double blocks = (double)((N + block - 1) / block) * Hkv;
+    double fa_parts = 1e30;
+    for (long n = 1; n <= 24 && (n == 1 || (n - 1) * 4 < tiles); ++n)
+      fa_parts = std::min(fa_parts, std::ceil(blocks * n / sms) * ((tiles + n - 1) / n * kFull[d] + 6) + 0.1 * n);
+    if (P == 0) fa_parts = 0;
+    const double units = (double)B * Hkv * (own_tiles + kSsItem);
+    const double own_us = stream ? units * std::max((d ? 0.66 : 0.33) / sms, d ? 0.0056 : 0.0028)
+                                 : std::max(own_tiles * kAlone[d][r], load * (own_tiles * kAmong[d][r] + 0.6)) + 3;
+    parts_us = 10 + std::max(fa_parts, own_us) + 0.35 * std::min(fa_parts, own_us) + (double)N * H * D * 16 / 2.5e6;
+  } else {
+    // in tile steps of an SM's two blocks; a join costs about one and a half
+    whole_us = std::ceil(load / 2) * all;
+    parts_us = ((rows + p.prefix_rows - 1) / p.prefix_rows * Hkv * tiles + own_blocks * own_tiles) / (2.0 * sms) + 1.5;
+    if (load < 1) whole_us = all;
+  }
+  p.fa_whole = fa_us < whole_us && fa_us < parts_us;
+  p.whole = !p.fa_whole && whole_us <= parts_us;
+  if (p.fa_whole) {
+    p.fa_ctas = (int)sms;
     p.list_cap = N / block + B;
     p.bytes = 16 + (size_t)p.list_cap * sizeof(int2);
     return p;
   }
-  p.prefix_rows = rows <= 16 ? 16 : 64;
-  p.own_rows = own <= 16 ? 16 : 64;
-  p.fa_prefix = bf && G <= 128 && rows >= 128 && P >= 512;
+  if (p.whole) {
+    p.own_parts = 1;
+    return p;
+  }
+  p.fa_prefix = tensor && P > 0;
   p.prefix_blocks = p.fa_prefix ? (N + block - 1) / block : (rows + p.prefix_rows - 1) / p.prefix_rows;
-  // enough blocks for two on every SM (one for the tensor-core kernel), no part under 256 keys
-  auto parts = [&](long want, long blocks, long most) {
-    return (int)std::max(1L, std::min(most, (want + blocks - 1) / std::max(1L, blocks)));
-  };
-  p.prefix_parts = P > 0 ? parts(p.fa_prefix ? sms : 2 * sms, p.prefix_blocks * Hkv, std::min(64L, (P + 255) / 256)) : 0;
-  const long own_blocks = (long)B * Hkv * ((own + p.own_rows - 1) / p.own_rows);
-  p.own_parts = parts(2 * sms, own_blocks, 16);
-  const int total = p.prefix_parts + p.own_parts;
-  if (total > 1) p.bytes = (size_t)total * N * H * (D * sizeof(float) + sizeof(float2));
+  if (p.fa_prefix && stream) {
+    // a tile step of the tensor-core kernel, and what an item costs beside its steps
+    const float step_us = (float)kFull[d] * 1.2f, item_us = 6.0f;
+    p.split.sms = (int)sms;
+    p.split.unit_us = D == 64 ? 0.33f : 0.66f;
+    p.split.floor_us = D == 64 ? 0.0028f : 0.0056f;
+    // candidates: n parts dealt in w even waves; kept where more blocks make the prefix a tenth faster
+    struct Choice {
+      int ctas, parts;
+      float us;
+    };
+    std::vector<Choice> all;
+    const long items1 = p.prefix_blocks * Hkv;
+    for (int n = 1; n <= 24 && (n == 1 || (n - 1) * 4 < tiles); ++n) {
+      const float item = (tiles + n - 1) / n * step_us + item_us;
+      for (int w = 1; w <= 8; ++w) {
+        const long c = (items1 * n + w - 1) / w;
+        if (c <= sms) all.push_back({(int)c, n, w * item + n * 0.1f});
+      }
+      const long w = (items1 * n + sms - 1) / sms;
+      all.push_back({(int)sms, n, w * item + n * 0.1f});
+    }
+    std::sort(all.begin(), all.end(), [](const Choice& x, const Choice& y) {
+      return x.ctas != y.ctas ? x.ctas < y.ctas : x.us < y.us;
+    });
+    for (float keep = 0.93f;; keep -= 0.05f) {
+      int n = 0;
+      float last = 0.f;
+      for (const Choice& c : all) {
+        if (n > 0 && c.us > keep * last) continue;
+        if (n > 0 && p.split.ctas[n - 1] == c.ctas) continue;
+        if (n < kSplits) p.split.ctas[n] = c.ctas, p.split.parts[n] = c.parts, p.split.fa_us[n] = c.us;
+        last = c.us;
+        ++n;
+      }
+      p.split.n = std::min(n, kSplits);
+      if (n <= kSplits || keep < 0.5f) break;
+    }
+    for (int i = 0; i < p.split.n; ++i) p.prefix_parts = std::max(p.prefix_parts, p.split.parts[i]);
+    p.fa_ctas = (int)sms;
+  } else if (p.fa_prefix) {
+    p.fa_ctas = (int)sms;
+    // waves of equal parts: the fewest tile steps on the busiest SM, a part costing two more
+    long best = 0;
+    for (int n = 1; n <= 64 && n * 4 <= tiles + 3; ++n) {
+      const long items = p.prefix_blocks * Hkv * n;
+      const long cost = (items + p.fa_ctas - 1) / p.fa_ctas * ((tiles + n - 1) / n + 2);
+      if (best == 0 || cost < best) best = cost, p.prefix_parts = n;
+    }
+  } else if (P > 0) {
+    // enough blocks for two on every SM, no part under 256 keys
+    const long blocks = p.prefix_blocks * Hkv;
+    p.prefix_parts = (int)std::max(1L, std::min(std::min(64L, (P + 255) / 256), (2 * sms + blocks - 1) / blocks));
+  }
+  if (stream) {
+    p.own_parts = 1;
+    p.cuts = (int)sms;
+  } else {
+    p.own_parts = (int)std::max(1L, std::min(16L, (2 * sms + (long)own_blocks - 1) / (long)own_blocks));
+  }
+  p.part_bytes = (size_t)(p.prefix_parts + p.own_parts) * N * H * (D * sizeof(float) + sizeof(float2));
+  p.part_bytes = (p.part_bytes + 15) / 16 * 16;
+  p.cut_bytes = (size_t)p.cuts * 32 * (D * sizeof(float) + sizeof(float2));
+  p.bytes = p.part_bytes + p.cut_bytes + (p.cuts ? (size_t)(B + 1) * sizeof(long) : 0);
   return p;
 }
 
@@ -592,8 +703,9 @@ int launch_sp_fa(const SpArgs& a, const SpPlan& p, int2* list, int* count, cudaS
     items = p.list_cap * a.Hkv;
     FCV_LAUNCH("sp_list_kernel", sp_list_kernel, dim3(1), dim3(1024), 0, s, a, block, list, f.list_cap, count);
   } else {
-    items = p.prefix_blocks * a.Hkv * p.prefix_parts;
+    items = p.prefix_blocks * a.Hkv * a.prefix_parts;
     f.prefix_items = (int)items;
+    f.prefix_blocks = (int)p.prefix_blocks;
   }
   static bool attr[64] = {false};
   int dev = 0;
@@ -602,7 +714,7 @@ int launch_sp_fa(const SpArgs& a, const SpPlan& p, int2* list, int* count, cudaS
     FCV_CUDA(cudaFuncSetAttribute(sp_fa_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, sf_smem_bytes<D>()));
     attr[dev & 63] = true;
   }
-  const int grid = (int)std::min(items, (long)num_sms());
+  const int grid = (int)std::min(items, (long)p.fa_ctas);
   FCV_LAUNCH("sp_fa_kernel", sp_fa_kernel<D>, dim3(grid), dim3(C::THREADS), sf_smem_bytes<D>(), s, tq, tpk, tpv, tk,
              tv, tv8, tv1, f);
   return FCV_OK;
@@ -624,16 +736,40 @@ int launch_sp_pieces(const SpArgs& a, dim3 grid, cudaStream_t s) {
   FCV_LAUNCH("sp_pieces_kernel", sp_pieces_kernel<T, D, RP, RO>, grid, dim3(sizeof(T) == 2 ? 128 : 256), smem, s, a);
   return FCV_OK;
 }
+// Own keys of a decode step, streamed (bf16, at most 16 stacked rows of a sequence in a row block).
+template <int D>
+int launch_sp_stream(const SpArgs& a, cudaStream_t s) {
+  using C = SpStream<D>;
+  const long cols = (long)a.Hkv * D;
+  CUtensorMap tq, tk, tv;
+  FCV_TRY(make_tmap_3d(&tq, a.q, D, a.H, a.N, D, a.q_stride, a.G, 16 / a.G));
+  FCV_TRY(make_tmap_bf16(&tk, a.k, a.kv_rows, cols, a.k_stride, kSpKeys));
+  FCV_TRY(make_tmap_bf16(&tv, a.v, a.kv_rows, cols, a.v_stride, kSpKeys));
+  static bool attr[64] = {false};
+  int dev = 0;
+  cudaGetDevice(&dev);
+  if (!attr[dev & 63]) {
+    FCV_CUDA(cudaFuncSetAttribute(sp_stream_kernel<D>, cudaFuncAttributeMaxDynamicSharedMemorySize, ss_smem_bytes<D>()));
+    attr[dev & 63] = true;
+  }
+  FCV_LAUNCH("sp_stream_kernel", sp_stream_kernel<D>, dim3(a.cuts), dim3(C::THREADS), ss_smem_bytes<D>(), s, tq, tk,
+             tv, a);
+  return FCV_OK;
+}
+
 template <typename T, int D>
 int run_sp(const SpArgs& a, const SpPlan& p, cudaStream_t s) {
   if (p.fa_prefix) FCV_TRY(launch_sp_fa<D>(a, p, nullptr, nullptr, s));
-  const long blocks = (long)a.prefix_items + (long)a.B * a.Hkv * a.own_parts;
-  if (blocks > 0x7fffffffL) return fail(FCV_EUNSUPPORTED, "fcv_shared_prefix_attention: too many blocks");
-  const dim3 grid((unsigned)blocks, (unsigned)a.own_rows);
-  if (p.prefix_rows == 16 && p.own_rows == 16) FCV_TRY((launch_sp_pieces<T, D, 16, 16>(a, grid, s)));
-  else if (p.own_rows == 16) FCV_TRY((launch_sp_pieces<T, D, 64, 16>(a, grid, s)));
-  else FCV_TRY((launch_sp_pieces<T, D, 64, 64>(a, grid, s)));
-  if (a.prefix_parts + a.own_parts > 1) {
+  if (a.cuts > 0) FCV_TRY(launch_sp_stream<D>(a, s));
+  const long blocks = (long)a.prefix_items + (a.cuts > 0 ? 0 : (long)a.B * a.Hkv * a.own_parts);
+  if (blocks > 0) {
+    if (blocks > 0x7fffffffL) return fail(FCV_EUNSUPPORTED, "fcv_shared_prefix_attention: too many blocks");
+    const dim3 grid((unsigned)blocks, (unsigned)(a.cuts > 0 ? 1 : a.own_rows));
+    if (p.prefix_rows == 16 && p.own_rows == 16) FCV_TRY((launch_sp_pieces<T, D, 16, 16>(a, grid, s)));
+    else if (p.own_rows == 16) FCV_TRY((launch_sp_pieces<T, D, 64, 16>(a, grid, s)));
+    else FCV_TRY((launch_sp_pieces<T, D, 64, 64>(a, grid, s)));
+  }
+  if (!a.whole) {
     const long warps = (long)a.N * a.H;
     FCV_LAUNCH("sp_join_kernel", sp_join_kernel<T, D>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, s, a);
   }
@@ -1168,9 +1304,10 @@ int fcv_qk_norm_rope(const void* qkv, int dtype, int N, long row_stride, int hea
                                  : run_qk_norm<float>(a, head_dim, interleaved != 0, s);
 }
 
-size_t fcv_shared_prefix_workspace_bytes(int N, int B, int heads, int kv_heads, int head_dim, int P, int dtype) {
-  if (!valid_dtype(dtype) || N <= 0 || B <= 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || P < 0) return 0;
-  return sp_plan(N, B, heads, kv_heads, head_dim, P, dtype == FCV_DTYPE_BF16).bytes;
+size_t fcv_shared_prefix_workspace_bytes(int N, int B, int heads, int kv_heads, int head_dim, int P, long kv_rows,
+                                         int packed, int dtype) {
+  if (!valid_dtype(dtype) || kv_rows < 0 || N <= 0 || B <= 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || P < 0) return 0;
+  return sp_plan(N, B, heads, kv_heads, head_dim, P, dtype == FCV_DTYPE_BF16, kv_rows, packed != 0).bytes;
 }
 
 int fcv_shared_prefix_attention(const void* q, long q_stride, const void* k, long k_stride, const void* v,
@@ -1200,7 +1337,7 @@ int fcv_shared_prefix_attention(const void* q, long q_stride, const void* k, lon
     return fail(FCV_EINVAL, "fcv_shared_prefix_attention: rows must be 16-byte aligned");
   if (P > 0x7fffff00 || kv_rows > 0x7fffff00L)  // row numbers of a tile past the last row stay 32-bit
     return fail(FCV_EUNSUPPORTED, "fcv_shared_prefix_attention: too many key rows");
-  const SpPlan p = sp_plan(N, B, heads, kv_heads, head_dim, P, dtype == FCV_DTYPE_BF16);
+  SpPlan p = sp_plan(N, B, heads, kv_heads, head_dim, P, dtype == FCV_DTYPE_BF16, kv_rows, !kv_lens);
   if (workspace_bytes < p.bytes || (p.bytes && !workspace) || (reinterpret_cast<uintptr_t>(workspace) & 15))
     return fail(FCV_EINVAL, "fcv_shared_prefix_attention: workspace of %zu bytes, %zu needed", workspace_bytes, p.bytes);
   if (p.prefix_blocks * kv_heads * p.prefix_parts > 0x7fffffffL)
@@ -1232,16 +1369,53 @@ int fcv_shared_prefix_attention(const void* q, long q_stride, const void* k, lon
   a.out_stride = out_stride;
   a.prefix_parts = p.prefix_parts;
   a.own_parts = p.own_parts;
+  a.whole = p.whole ? 1 : 0;
+  a.beside = p.fa_prefix && pdl_enabled() ? 1 : 0;
   a.prefix_items = p.fa_prefix ? 0 : (int)(p.prefix_blocks * kv_heads * p.prefix_parts);
   cudaStream_t s = as_stream(stream);
-  if (p.whole) {
+  if (p.fa_whole) {
     int* count = static_cast<int*>(workspace);
     int2* list = reinterpret_cast<int2*>(count + 4);
     return head_dim == 64 ? launch_sp_fa<64>(a, p, list, count, s) : launch_sp_fa<128>(a, p, list, count, s);
   }
   const long own = ((long)N + B - 1) / B * a.G;
   a.own_rows = (int)std::min(1024L, (own + p.own_rows - 1) / p.own_rows);
+  a.cuts = p.cuts;
+  a.split = p.split;
+  if (a.split.n) {
+    a.split.floor_us = std::max(p.split.floor_us, p.split.unit_us / num_sms());
+    for (int i = 0; i < a.split.n; ++i) {
+      const int left = a.split.sms - a.split.ctas[i];
+      a.split.own_us[i] = left > 0 ? std::max(p.split.floor_us, p.split.unit_us / left) : 0.f;
+    }
+    // A short prefix is given the few SMs on which it takes no longer than the own keys could (by the
+    // rows of k, at most 30 us): the device's choice costs 6 us (64 streams behind 4096 keys: 50 us
+    // against 44), and being wrong costs little.
+    const float units = (float)kv_rows * kv_heads / kSpKeys + (float)B * kv_heads * (kSsItem + 1);
+    const float most = std::min(30.f, std::max(12.f, 8.f + units * a.split.floor_us));
+    for (int i = 0; i < a.split.n; ++i) {
+      if (a.split.fa_us[i] > most) continue;
+      if (3 * a.split.ctas[i] > a.split.sms) break;
+      a.prefix_parts = a.split.parts[i];
+      p.fa_ctas = a.split.ctas[i];
+      a.cuts = a.split.sms - p.fa_ctas;
+      a.split.n = 0;
+      break;
+    }
+  }
+  if (kv_rows == 0 && p.cuts) {  // no own keys at all: nothing to stream, and the join finds no own part
+    a.cuts = 0;
+    a.own_parts = 0;
+    if (a.split.n) a.prefix_parts = a.split.parts[a.split.n - 1];
+    a.split.n = 0;
+  }
   const size_t rows = (size_t)(p.prefix_parts + p.own_parts) * N * heads;
+  if (a.cuts) {
+    char* at = static_cast<char*>(workspace) + p.part_bytes;
+    a.cut_o = reinterpret_cast<float*>(at);
+    a.cut_ml = reinterpret_cast<float2*>(a.cut_o + (size_t)a.cuts * 32 * head_dim);
+    a.tile_start = reinterpret_cast<long*>(at + p.cut_bytes);
+  }
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(static_cast<float*>(workspace) + rows * head_dim);
   if (dtype == FCV_DTYPE_BF16)

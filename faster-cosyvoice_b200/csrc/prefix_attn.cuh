@@ -20,6 +20,21 @@
 
 namespace fcv {
 
+// How the SMs are shared between the prefix parts (tensor-core kernel) and the own keys
+// (sp_stream_kernel) of a decode step: the choices that the host worked out, each with the blocks and
+// parts of the former and its time.  The own keys are known on the device only, so each kernel picks
+// the same choice from their number (sp_pick).
+constexpr int kSplits = 12;
+struct SpSplit {
+  int n;                 // 0: prefix_parts and cuts are fixed
+  int sms;
+  int ctas[kSplits], parts[kSplits];
+  float fa_us[kSplits];  // time of the prefix parts
+  float own_us[kSplits]; // time of a unit of own keys beside them (0: no SM is left, they come after)
+  float unit_us;         // a unit of own keys on one SM,
+  float floor_us;        // and on the whole GPU (memory bandwidth)
+};
+
 struct SpArgs {
   const void* q;
   long q_stride;  // elements between query rows; heads are D apart
@@ -40,8 +55,18 @@ struct SpArgs {
   long out_stride;
   float* part_o;   // (parts, N, H, D)
   float2* part_ml; // (parts, N, H): maximum (log2 units) and sum
-  int prefix_parts, own_parts;  // one part in all: written to out, nothing to join
-  int prefix_items, own_rows;   // blocks of the prefix; blockIdx.y slots of a sequence's row blocks
+  int prefix_parts, own_parts;
+  int prefix_items;  // blocks of the prefix
+  int own_rows;      // blockIdx.y slots of a sequence's row blocks
+  int whole;         // a sequence's rows take the prefix and their own keys in one go: nothing to join
+  int beside;        // runs beside the kernel launched before it (see sp_pieces_kernel)
+  // own keys by sp_stream_kernel (prefix_stream.cuh): cuts > 0 stretches, the tiles before every
+  // sequence (B + 1), and two boundary slots of 16 rows for every stretch
+  int cuts;
+  long* tile_start;
+  float* cut_o;
+  float2* cut_ml;
+  SpSplit split;
 };
 
 constexpr int kSpKeys = 64;  // keys of a tile
@@ -51,32 +76,36 @@ struct SpSeq {
   long base;
 };
 // The device arrays of a sequence, checked: rows outside the buffers are never touched.
-__device__ __forceinline__ SpSeq sp_sequence(const SpArgs& a, int b) {
+__device__ __forceinline__ SpSeq sp_sequence(const SpArgs& a, int b, bool report) {
   SpSeq s;
   const int c0 = a.cu[b], c1 = a.cu[b + 1];
   s.q0 = c0;
   s.nq = c1 - c0;
   if (c0 < 0 || c1 < c0 || c1 > a.N) {
-    if (threadIdx.x == 0) record_error(611);
+    if (report) record_error(611);
     s.q0 = 0;
     s.nq = 0;
   }
   s.base = a.kv_base ? a.kv_base[b] : s.q0;
   s.nk = a.kv_lens ? a.kv_lens[b] : s.nq;
   if (s.nk < 0 || s.base < 0 || s.base + s.nk > a.kv_rows) {
-    if (s.nk != 0 && threadIdx.x == 0) record_error(612);
+    if (s.nk != 0 && report) record_error(612);
     s.base = 0;
     s.nk = 0;
   }
   return s;
 }
+// Own keys, of nk, that a query at own position `at` sees (negative: before the first own key).
+__device__ __forceinline__ int sp_limit_at(const SpArgs& a, int nk, int at) {
+  if (a.chunk <= 0) return nk;
+  const long pos = (long)a.P + at;
+  if (pos < 0) return 0;
+  const long lim = a.chunk == 1 ? (long)at + 1 : (pos / a.chunk + 1) * a.chunk - a.P;
+  return lim < 0 ? 0 : (lim < nk ? static_cast<int>(lim) : nk);
+}
 // Own keys that query i of the sequence sees.
 __device__ __forceinline__ int sp_limit(const SpArgs& a, const SpSeq& s, int i) {
-  if (a.chunk <= 0) return s.nk;
-  const long at = (long)a.P + s.nk - s.nq + i;
-  if (at < 0) return 0;
-  const long lim = (at / a.chunk + 1) * a.chunk - a.P;
-  return lim < 0 ? 0 : (lim < s.nk ? static_cast<int>(lim) : s.nk);
+  return sp_limit_at(a, s.nk, s.nk - s.nq + i);
 }
 // Tiles [t0, t1) of piece `part` out of at most `parts` over `tiles` tiles: pieces of equal size,
 // none shorter than four tiles unless it is the last.
@@ -86,6 +115,15 @@ __device__ __forceinline__ void sp_piece(int tiles, int parts, int part, int& t0
   t0 = min(tiles, part * each);
   t1 = part < n ? min(tiles, t0 + each) : t0;
 }
+
+// A stretch of keys of one key head: tiles [t0, t1) of the rows of k / v, of which the first kend exist.
+template <typename T>
+struct SpKeys {
+  const T* k;
+  const T* v;
+  long ks, vs;  // row strides
+  int kend, t0, t1;
+};
 
 __device__ __forceinline__ void cp_async16(uint32_t dst, const void* src, bool valid) {
   const int n = valid ? 16 : 0;  // 0: the 16 bytes are zeroed, the source is not read
@@ -138,17 +176,18 @@ struct SpMma {
   static constexpr int kSmem = kQ + kStages * 2 * kTile;
 };
 
-// One piece: stacked rows [R0, R0 + rows) of key head hk (rows <= 16 WM) against key rows
-// [0, kend) of K / V, tiles [t0, t1).  4 warps: WM of them along the rows (16 each), 4 / WM along
-// the keys of a tile; for WM < 4 the warps' partial results are joined in shared memory.
-//   limits: row r of the block sees keys [0, lim(r)).
+// One piece: stacked rows [R0, R0 + rows) of key head hk (rows <= 16 WM) against the tiles of `pre`
+// (keys that every row sees) and then of `own` (row r of the block sees keys [0, limit(r))).  The
+// result is part `part` of the rows, or final for part < 0.  4 warps: WM of them along the rows (16
+// each), 4 / WM along the keys of a tile; for WM < 4 the warps' partial results are joined in shared
+// memory.
 // K, V tiles come by 16-byte asynchronous copies into a ring; a row of a tile is D / 8 chunks of
 // 16 bytes, chunk c of row r at c ^ (r % 8), which keeps ldmatrix free of bank conflicts.
-// Rows past kend are zero in shared memory, so stale values behind a sequence never reach a product.
+// Rows past the last key are zero in shared memory, so stale values behind a sequence never reach a product.
 template <int D, int WM, typename Limit>
-__device__ __forceinline__ void sp_mma_piece(const SpArgs& a, uint8_t* smem, const bf16* K, const bf16* V,
-                                             long k_stride, long v_stride, int hk, long R0, int rows, int kend,
-                                             int t0, int t1, int part, Limit limit) {
+__device__ __forceinline__ void sp_mma_piece(const SpArgs& a, uint8_t* smem, const SpKeys<bf16>& pre,
+                                             const SpKeys<bf16>& own, int hk, long R0, int rows, int part,
+                                             Limit limit) {
   using C = SpMma<D>;
   constexpr int WK = 4 / WM;
   constexpr int KW = kSpKeys / WK;  // keys of a tile that a warp takes
@@ -157,7 +196,8 @@ __device__ __forceinline__ void sp_mma_piece(const SpArgs& a, uint8_t* smem, con
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
   const int wm = warp % WM, wk = warp / WM;
   const uint32_t s0 = smem_u32(smem), sQ = s0, sKV = s0 + C::kQ;
-  const bool direct = a.prefix_parts + a.own_parts == 1;
+  const bool direct = part < 0;
+  const int n_pre = pre.t1 - pre.t0, tiles = n_pre + own.t1 - own.t0;
 
   auto put = [&](uint32_t base, int r, int c) { return base + r * (D * 2) + ((c ^ (r & 7)) << 4); };
   __syncthreads();  // an earlier piece of this block has left the buffers
@@ -167,21 +207,25 @@ __device__ __forceinline__ void sp_mma_piece(const SpArgs& a, uint8_t* smem, con
     const SpRow x = sp_row(a, hk, R0 + (ok ? r : 0));
     cp_async16(put(sQ, r, c), static_cast<const bf16*>(a.q) + x.token * a.q_stride + (long)x.head * D + 8 * c, ok);
   }
-  auto load = [&](int t) {
-    const uint32_t kb = sKV + ((t - t0) % STAGES) * 2 * C::kTile, vb = kb + C::kTile;
+  const int lr = tid / CH, lc = tid % CH;  // this thread copies chunk lc of rows lr, lr + 128 / CH, ...
+  auto load = [&](int u) {
+    const bool first = u < n_pre;
+    const SpKeys<bf16>& src = first ? pre : own;
+    const int key = (src.t0 + (first ? u : u - n_pre)) * kSpKeys + lr;
+    const uint32_t kb = sKV + (u % STAGES) * 2 * C::kTile, vb = kb + C::kTile;
+    const bf16* kp = src.k + key * src.ks + 8 * lc;
+    const bf16* vp = src.v + key * src.vs + 8 * lc;
 #pragma unroll
-    for (int i = tid; i < kSpKeys * CH; i += 128) {
-      const int r = i / CH, c = i % CH;
-      const long key = (long)t * kSpKeys + r;
-      const bool ok = key < kend;
-      const long at = ok ? key : 0;
-      cp_async16(put(kb, r, c), K + at * k_stride + 8 * c, ok);
-      cp_async16(put(vb, r, c), V + at * v_stride + 8 * c, ok);
+    for (int j = 0; j < kSpKeys * CH / 128; ++j) {
+      constexpr int step = 128 / CH;
+      const bool ok = key + j * step < src.kend;
+      cp_async16(put(kb, lr + j * step, lc), ok ? kp + j * step * src.ks : src.k, ok);
+      cp_async16(put(vb, lr + j * step, lc), ok ? vp + j * step * src.vs : src.v, ok);
     }
   };
 #pragma unroll
   for (int i = 0; i < STAGES - 1; ++i) {
-    if (t0 + i < t1) load(t0 + i);
+    if (i < tiles) load(i);
     cp_async_commit();
   }
 
@@ -194,17 +238,17 @@ __device__ __forceinline__ void sp_mma_piece(const SpArgs& a, uint8_t* smem, con
   for (int i = 0; i < D / 8; ++i) o[i][0] = o[i][1] = o[i][2] = o[i][3] = 0.f;
   uint32_t qf[D / 16][4];
 
-  for (int t = t0; t < t1; ++t) {
+  for (int t = 0; t < tiles; ++t) {
     cp_async_wait<STAGES - 2>();
     __syncthreads();
-    if (t + STAGES - 1 < t1) load(t + STAGES - 1);
+    if (t + STAGES - 1 < tiles) load(t + STAGES - 1);
     cp_async_commit();
-    if (t == t0) {
+    if (t == 0) {
 #pragma unroll
       for (int kk = 0; kk < D / 16; ++kk)
         ldsm4(put(sQ, 16 * wm + (lane & 15), 2 * kk + (lane >> 4)), qf[kk][0], qf[kk][1], qf[kk][2], qf[kk][3]);
     }
-    const uint32_t kb = sKV + ((t - t0) % STAGES) * 2 * C::kTile, vb = kb + C::kTile;
+    const uint32_t kb = sKV + (t % STAGES) * 2 * C::kTile, vb = kb + C::kTile;
     float s[KW / 8][4];
 #pragma unroll
     for (int i = 0; i < KW / 8; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
@@ -219,15 +263,16 @@ __device__ __forceinline__ void sp_mma_piece(const SpArgs& a, uint8_t* smem, con
         mma_bf16(s[2 * nb + 1], qf[kk], b2, b3);
       }
     }
-    const int k0 = t * kSpKeys + wk * KW;
-    if (wmin < k0 + KW) {  // some row of the warp stops inside this warp's keys
-      const int c0 = k0 + 2 * (lane & 3);
+    const bool first = t < n_pre;
+    const int k0 = (first ? pre.t0 + t : own.t0 + t - n_pre) * kSpKeys + wk * KW;
+    if ((first ? pre.kend : wmin) < k0 + KW) {  // some row of the warp stops inside this warp's keys
+      const int c0 = k0 + 2 * (lane & 3), z0 = first ? pre.kend : lim0, z1 = first ? pre.kend : lim1;
 #pragma unroll
       for (int i = 0; i < KW / 8; ++i) {
 #pragma unroll
         for (int j = 0; j < 2; ++j) {
-          if (c0 + 8 * i + j >= lim0) s[i][j] = -INFINITY;
-          if (c0 + 8 * i + j >= lim1) s[i][2 + j] = -INFINITY;
+          if (c0 + 8 * i + j >= z0) s[i][j] = -INFINITY;
+          if (c0 + 8 * i + j >= z1) s[i][2 + j] = -INFINITY;
         }
       }
     }
@@ -367,16 +412,17 @@ struct SpF32 {
   static constexpr int kSmem = 4 * (kRows * kLd + kStages * 2 * kSpKeys * kLd + kRows * (kSpKeys + 4));
 };
 template <int D, int RPT, typename Limit>
-__device__ __forceinline__ void sp_f32_piece(const SpArgs& a, uint8_t* smem, const float* K, const float* V,
-                                             long k_stride, long v_stride, int hk, long R0, int rows, int kend,
-                                             int t0, int t1, int part, Limit limit) {
+__device__ __forceinline__ void sp_f32_piece(const SpArgs& a, uint8_t* smem, const SpKeys<float>& pre,
+                                             const SpKeys<float>& own, int hk, long R0, int rows, int part,
+                                             Limit limit) {
   using C = SpF32<D, RPT>;
   constexpr int LD = C::kLd, CH = D / 4, PLD = kSpKeys + 4;
   float* sQ = reinterpret_cast<float*>(smem);
   float* sKV = sQ + C::kRows * LD;
   float* sP = sKV + C::kStages * 2 * kSpKeys * LD;
   const int tid = threadIdx.x, tx = tid & 15, ty = tid >> 4;
-  const bool direct = a.prefix_parts + a.own_parts == 1;
+  const bool direct = part < 0;
+  const int n_pre = pre.t1 - pre.t0, tiles = n_pre + own.t1 - own.t0;
   __syncthreads();
   for (int i = tid; i < C::kRows * CH; i += 256) {
     const int r = i / CH, c = i % CH;
@@ -385,19 +431,24 @@ __device__ __forceinline__ void sp_f32_piece(const SpArgs& a, uint8_t* smem, con
     cp_async16(smem_u32(sQ + r * LD + 4 * c),
                static_cast<const float*>(a.q) + x.token * a.q_stride + (long)x.head * D + 4 * c, ok);
   }
-  auto load = [&](int t) {
-    float* kb = sKV + ((t - t0) & 1) * 2 * kSpKeys * LD;
+  const int lr = tid / CH, lc = tid % CH;  // this thread copies chunk lc of rows lr, lr + 256 / CH, ...
+  auto load = [&](int u) {
+    const bool first = u < n_pre;
+    const SpKeys<float>& src = first ? pre : own;
+    const int key = (src.t0 + (first ? u : u - n_pre)) * kSpKeys + lr;
+    float* kb = sKV + (u & 1) * 2 * kSpKeys * LD + lr * LD + 4 * lc;
     float* vb = kb + kSpKeys * LD;
-    for (int i = tid; i < kSpKeys * CH; i += 256) {
-      const int r = i / CH, c = i % CH;
-      const long key = (long)t * kSpKeys + r;
-      const bool ok = key < kend;
-      const long at = ok ? key : 0;
-      cp_async16(smem_u32(kb + r * LD + 4 * c), K + at * k_stride + 4 * c, ok);
-      cp_async16(smem_u32(vb + r * LD + 4 * c), V + at * v_stride + 4 * c, ok);
+    const float* kp = src.k + key * src.ks + 4 * lc;
+    const float* vp = src.v + key * src.vs + 4 * lc;
+#pragma unroll
+    for (int j = 0; j < kSpKeys * CH / 256; ++j) {
+      constexpr int step = 256 / CH;
+      const bool ok = key + j * step < src.kend;
+      cp_async16(smem_u32(kb + j * step * LD), ok ? kp + j * step * src.ks : src.k, ok);
+      cp_async16(smem_u32(vb + j * step * LD), ok ? vp + j * step * src.vs : src.v, ok);
     }
   };
-  if (t0 < t1) load(t0);
+  if (tiles > 0) load(0);
   cp_async_commit();
   int lim[RPT];
   float m[RPT], l[RPT];
@@ -410,12 +461,12 @@ __device__ __forceinline__ void sp_f32_piece(const SpArgs& a, uint8_t* smem, con
 #pragma unroll
     for (int d = 0; d < D / 16; ++d) o[i][d] = 0.f;
   }
-  for (int t = t0; t < t1; ++t) {
+  for (int t = 0; t < tiles; ++t) {
     cp_async_wait<0>();
     __syncthreads();
-    if (t + 1 < t1) load(t + 1);
+    if (t + 1 < tiles) load(t + 1);
     cp_async_commit();
-    const float* kb = sKV + ((t - t0) & 1) * 2 * kSpKeys * LD;
+    const float* kb = sKV + (t & 1) * 2 * kSpKeys * LD;
     const float* vb = kb + kSpKeys * LD;
     float s[RPT][4];
 #pragma unroll
@@ -437,13 +488,15 @@ __device__ __forceinline__ void sp_f32_piece(const SpArgs& a, uint8_t* smem, con
         }
       }
     }
-    const int k0 = t * kSpKeys + tx;
+    const bool first = t < n_pre;
+    const int k0 = (first ? pre.t0 + t : own.t0 + t - n_pre) * kSpKeys + tx;
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
       float x = -INFINITY;
+      const int z = first ? pre.kend : lim[i];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        s[i][j] = k0 + 16 * j < lim[i] ? s[i][j] * a.scale_log2 : -INFINITY;
+        s[i][j] = k0 + 16 * j < z ? s[i][j] * a.scale_log2 : -INFINITY;
         x = fmaxf(x, s[i][j]);
       }
 #pragma unroll
@@ -517,24 +570,26 @@ __device__ __forceinline__ void sp_f32_piece(const SpArgs& a, uint8_t* smem, con
 // ------------------------------------------------------------------ the pieces of a call
 // Blocks [0, prefix_items): (row block, key head, part) of the prefix over the stacked rows of the
 // batch.  The others: (sequence, key head, part) of the own keys, blockIdx.y striding over the row
-// blocks of the sequence.  RP / RO: rows of a block of the prefix / of a sequence; they set the
-// shape of the block (see the piece functions).
+// blocks of the sequence; with `whole` they take the prefix as well.  RP / RO: rows of a block of
+// the prefix / of a sequence; they set the shape of the block (see the piece functions).
+// `beside`: the tensor-core kernel of the prefix parts was launched just before on a part of the
+// SMs, and this kernel fills the others.  Every block of that kernel has waited for the work before
+// it when this one starts, and its results are not read here, so the wait moves to the end, where
+// it makes this kernel's completion imply the other's.
 template <typename T, int D, int RP, int RO>
-__global__ void __launch_bounds__(sizeof(T) == 2 ? 128 : 256) sp_pieces_kernel(const SpArgs a) {
-  griddep_wait();
-  griddep_launch();
-  extern __shared__ __align__(128) uint8_t smem[];
-  auto piece = [&](auto rows_c, const void* K, const void* V, long ks, long vs, int hk, long R0, int rows, int kend,
-                   int t0, int t1, int part, auto limit) {
+__device__ __forceinline__ void sp_block(const SpArgs& a, uint8_t* smem) {
+  auto piece = [&](auto rows_c, const SpKeys<T>& pre, const SpKeys<T>& own, int hk, long R0, int rows, int part,
+                   auto limit) {
     constexpr int R = decltype(rows_c)::value;
-    const T* k = static_cast<const T*>(K) + (long)hk * D;
-    const T* v = static_cast<const T*>(V) + (long)hk * D;
     if constexpr (sizeof(T) == 2)
-      sp_mma_piece<D, R / 16>(a, smem, k, v, ks, vs, hk, R0, rows, kend, t0, t1, part, limit);
+      sp_mma_piece<D, R / 16>(a, smem, pre, own, hk, R0, rows, part, limit);
     else
-      sp_f32_piece<D, R / 16>(a, smem, k, v, ks, vs, hk, R0, rows, kend, t0, t1, part, limit);
+      sp_f32_piece<D, R / 16>(a, smem, pre, own, hk, R0, rows, part, limit);
   };
   int it = blockIdx.x;
+  SpKeys<T> pre{static_cast<const T*>(a.pk), static_cast<const T*>(a.pv), a.pk_stride, a.pv_stride, a.P, 0, 0};
+  SpKeys<T> own{static_cast<const T*>(a.k), static_cast<const T*>(a.v), a.k_stride, a.v_stride, 0, 0, 0};
+  const int prefix_tiles = (a.P + kSpKeys - 1) / kSpKeys;
   if (it < a.prefix_items) {
     if (blockIdx.y != 0) return;
     const int part = it % a.prefix_parts;
@@ -545,60 +600,207 @@ __global__ void __launch_bounds__(sizeof(T) == 2 ? 128 : 256) sp_pieces_kernel(c
     const long r0 = R0 > first ? R0 : first;
     const long r1 = min(R0 + RP, end);
     if (r0 >= r1) return;
-    int t0, t1;
-    sp_piece((a.P + kSpKeys - 1) / kSpKeys, a.prefix_parts, part, t0, t1);
-    const int P = a.P;
-    piece(std::integral_constant<int, RP>(), a.pk, a.pv, a.pk_stride, a.pv_stride, hk, r0, static_cast<int>(r1 - r0),
-          P, t0, t1, part, [P](int) { return P; });
+    sp_piece(prefix_tiles, a.prefix_parts, part, pre.t0, pre.t1);
+    pre.k += (long)hk * D;
+    pre.v += (long)hk * D;
+    piece(std::integral_constant<int, RP>(), pre, own, hk, r0, static_cast<int>(r1 - r0), part,
+          [](int) { return 0; });
     return;
   }
   it -= a.prefix_items;
   const int part = it % a.own_parts;
   it /= a.own_parts;
   const int hk = it % a.Hkv, b = it / a.Hkv;
-  const SpSeq s = sp_sequence(a, b);
+  const SpSeq s = sp_sequence(a, b, threadIdx.x == 0);
   const long nrows = (long)s.nq * a.G;
+  pre.k += (long)hk * D;
+  pre.v += (long)hk * D;
+  own.k += s.base * a.k_stride + (long)hk * D;
+  own.v += s.base * a.v_stride + (long)hk * D;
+  own.kend = s.nk;
+  if (a.whole) pre.t1 = prefix_tiles;
   for (long r = (long)blockIdx.y * RO; r < nrows; r += (long)gridDim.y * RO) {
     const int rows = static_cast<int>(min((long)RO, nrows - r));
     const int seen = sp_limit(a, s, static_cast<int>((r + rows - 1) / a.G));  // limits grow along the rows
-    int t0, t1;
-    sp_piece((seen + kSpKeys - 1) / kSpKeys, a.own_parts, part, t0, t1);
-    piece(std::integral_constant<int, RO>(), static_cast<const T*>(a.k) + s.base * a.k_stride,
-          static_cast<const T*>(a.v) + s.base * a.v_stride, a.k_stride, a.v_stride, hk, (long)s.q0 * a.G + r, rows,
-          s.nk, t0, t1, a.prefix_parts + part,
+    sp_piece((seen + kSpKeys - 1) / kSpKeys, a.own_parts, part, own.t0, own.t1);
+    piece(std::integral_constant<int, RO>(), pre, own, hk, (long)s.q0 * a.G + r, rows,
+          a.whole ? -1 : a.prefix_parts + part,
           [&](int i) { return sp_limit(a, s, static_cast<int>((r + i) / a.G)); });
   }
 }
+template <typename T, int D, int RP, int RO>
+__global__ void __launch_bounds__(sizeof(T) == 2 ? 128 : 256) sp_pieces_kernel(const SpArgs a) {
+  extern __shared__ __align__(128) uint8_t smem[];
+  if (!a.beside) griddep_wait();
+  griddep_launch();
+  sp_block<T, D, RP, RO>(a, smem);
+  if (a.beside) griddep_wait();
+}
 
-// Joins the parts of a row: one warp per (token, head).
+// Own parts left by sp_stream_kernel.  The (sequence, row block, key head) items lie end to end, each
+// kSsItem units for its own cost and one for every key tile, and are cut into equal stretches.
+constexpr int kSsItem = 3;
+struct SsCount {
+  int blocks, tiles;  // row blocks of 16 / G tokens; key tiles of each item
+  __device__ __forceinline__ int units() const { return tiles > 0 ? tiles + kSsItem : 0; }
+  __device__ __forceinline__ long all(int Hkv) const { return (long)blocks * Hkv * units(); }
+};
+__device__ __forceinline__ SsCount ss_count(const SpArgs& a, int nq, int nk) {
+  const int per = 16 / a.G;
+  SsCount c;
+  c.blocks = (nq + per - 1) / per;
+  c.tiles = (nk + kSpKeys - 1) / kSpKeys;
+  return c;
+}
+// Stretches of `total` units (none is empty), the first unit of stretch c, the stretch that holds a unit.
+__device__ __forceinline__ int ss_stretches(long total, int cuts) {
+  return static_cast<int>(min(total, (long)cuts));
+}
+__device__ __forceinline__ long ss_cut(long total, int n, long c) { return total * c / n; }
+__device__ __forceinline__ int ss_stretch(long total, int n, long unit) {
+  return static_cast<int>(((unit + 1) * n - 1) / total);
+}
+
+// The choice whose slower side is the fastest for `units` of own keys.
+__device__ __forceinline__ int sp_pick(const SpSplit& s, long units) {
+  int best = 0;
+  float best_us = 0.f;
+  const float u = static_cast<float>(units);
+  for (int i = 0; i < s.n; ++i) {
+    const float us = s.own_us[i] > 0.f ? fmaxf(s.fa_us[i], u * s.own_us[i]) : s.fa_us[i] + u * s.floor_us;
+    if (i == 0 || us < best_us) best = i, best_us = us;
+  }
+  return best;
+}
+__device__ __forceinline__ int sp_pick_cuts(const SpSplit& s, int i) {
+  return s.ctas[i] < s.sms ? s.sms - s.ctas[i] : s.sms;
+}
+
+// Joins the parts of a row: one warp per (token, head).  Its loads are a chain of round trips (the
+// token's sequence, the parts' maxima and sums, their outputs), so what can be read at once is.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) sp_join_kernel(const SpArgs a) {
   griddep_wait();
   griddep_launch();
   const int lane = threadIdx.x & 31;
   const long w = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const long token = w / a.H;
-  if (token >= a.N || token < a.cu[0] || token >= a.cu[a.B]) return;  // rows behind the last sequence stay
-  const int parts = a.prefix_parts + a.own_parts;
+  const int token = static_cast<int>(w / a.H);
+  if (token >= a.N) return;
+  const int head = static_cast<int>(w - (long)token * a.H);
   const long step = (long)a.N * a.H;
-  float m = -INFINITY;
-  for (int p = 0; p < parts; ++p) m = fmaxf(m, a.part_ml[p * step + w].x);
+  // own parts: all of them, or (cuts) one in the row's own place or one in each stretch that the item meets
+  int own = a.own_parts, first = -1, prefix_parts = a.prefix_parts;
+  long slot_row = 0;
+  const int begin = a.cu[0], end = a.cu[a.B];
+  if (a.cuts > 0) {
+    own = 0;
+    // the token's sequence: its own number when every sequence has one query
+    int b = min(token, a.B - 1);
+    SpSeq s = sp_sequence(a, b, false);
+    long start = a.tile_start[b];
+    const long total = a.tile_start[a.B];
+    if (s.q0 > token || s.q0 + s.nq <= token) {
+      int lo = 0, hi = a.B - 1;
+      while (lo < hi) {
+        const int mid = (lo + hi) / 2;
+        if (a.cu[mid + 1] > token) hi = mid;
+        else lo = mid + 1;
+      }
+      s = sp_sequence(a, lo, false);
+      start = a.tile_start[lo];
+    }
+    const SsCount c = ss_count(a, s.nq, s.nk);
+    const int i = token - s.q0;
+    int cuts = a.cuts;
+    if (a.split.n > 0) {
+      const int pick = sp_pick(a.split, total);
+      cuts = sp_pick_cuts(a.split, pick);
+      prefix_parts = a.split.parts[pick];
+    }
+    if (i >= 0 && i < s.nq && c.tiles > 0) {
+      const int per = 16 / a.G, hk = head / a.G, rb = i / per;
+      start += (long)(rb * a.Hkv + hk) * c.units() + kSsItem;  // the item's first tile
+      const int n = ss_stretches(total, cuts);
+      const int c0 = ss_stretch(total, n, start), c1 = ss_stretch(total, n, start + c.tiles - 1);
+      own = c1 - c0 + 1;
+      if (own > 1) first = c0;
+      slot_row = (i - rb * per) * a.G + (head - hk * a.G);
+    }
+  }
+  if (token < begin || token >= end) return;  // rows behind the last sequence stay
+  const int parts = prefix_parts + own;
+  // part p of the row: its index among the stored maxima and sums (and, times D, among the outputs)
+  auto place = [&](int p, const float2*& ml, const float*& o) {
+    if (p >= prefix_parts && first >= 0) {
+      const int c = first + p - prefix_parts;
+      // a stretch keeps the item that began before it in slot 0, the one that goes on behind it in slot 1
+      const long at = (2L * c + (c == first ? 1 : 0)) * 16 + slot_row;
+      ml = a.cut_ml + at;
+      o = a.cut_o + at * D;
+    } else {
+      // own part 0 stands behind the places of a.prefix_parts parts, of which fewer may be in use
+      const long at = (p < prefix_parts ? p : a.prefix_parts + p - prefix_parts) * step + w;
+      ml = a.part_ml + at;
+      o = a.part_o + at * D;
+    }
+  };
+  // 32 parts at a time: lane p has part p's maximum, sum and place; the outputs are then read by the
+  // whole warp, eight parts in flight
   constexpr int V = D / 32;
   float acc[V];
 #pragma unroll
   for (int i = 0; i < V; ++i) acc[i] = 0.f;
-  float l = 0.f;
-  for (int p = 0; p < parts; ++p) {
-    const float2 ml = a.part_ml[p * step + w];
-    if (ml.x == -INFINITY && ml.y == 0.f) continue;
-    const float f = exp2f(ml.x - m);
-    l = fmaf(ml.y, f, l);
-    const float* src = a.part_o + (p * step + w) * D + V * lane;
+  float m = -INFINITY, l = 0.f;
+  for (int p0 = 0; p0 < parts; p0 += 32) {
+    const int n = min(32, parts - p0);
+    float2 ml = make_float2(-INFINITY, 0.f);
+    const float* o = nullptr;
+    if (lane < n) {
+      const float2* at;
+      place(p0 + lane, at, o);
+      ml = *at;
+    }
+    float top = ml.x;
 #pragma unroll
-    for (int i = 0; i < V; ++i) acc[i] = fmaf(src[i], f, acc[i]);
+    for (int i = 16; i > 0; i >>= 1) top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, i));
+    const float m_new = fmaxf(m, top);
+    if (m_new > m) {  // rescale what the parts before left
+      const float f = exp2f(m - m_new);
+      l *= f;
+#pragma unroll
+      for (int i = 0; i < V; ++i) acc[i] *= f;
+      m = m_new;
+    }
+    // a part that saw no key (maximum -inf, sum 0) holds no output; a sum that is NaN is kept
+    const bool some = ml.x != -INFINITY || ml.y != 0.f;
+    const float f = !some ? 0.f : (m == -INFINITY ? 1.f : exp2f(ml.x - m));
+    float part = some ? ml.y * f : 0.f;
+#pragma unroll
+    for (int i = 16; i > 0; i >>= 1) part += __shfl_xor_sync(0xffffffffu, part, i);
+    l += part;
+    uint32_t todo = __ballot_sync(0xffffffffu, some);
+    while (todo) {
+      float v[8][V], g[8];
+#pragma unroll
+      for (int u = 0; u < 8; ++u) {
+        const int p = todo ? __ffs(todo) - 1 : 0;
+        const bool have = todo != 0;
+        todo &= todo - 1;
+        g[u] = __shfl_sync(0xffffffffu, f, p);
+        const unsigned long long at = __shfl_sync(0xffffffffu, reinterpret_cast<unsigned long long>(o), p);
+        const float* src = reinterpret_cast<const float*>(at) + V * lane;
+#pragma unroll
+        for (int i = 0; i < V; ++i) v[u][i] = have ? src[i] : 0.f;
+        if (!have) g[u] = 0.f;
+      }
+#pragma unroll
+      for (int u = 0; u < 8; ++u)
+#pragma unroll
+        for (int i = 0; i < V; ++i) acc[i] = fmaf(v[u][i], g[u], acc[i]);
+    }
   }
   const float inv = l > 0.f || l != l ? 1.f / l : 0.f;
-  T* dst = static_cast<T*>(a.out) + token * a.out_stride + (w - token * a.H) * D + V * lane;
+  T* dst = static_cast<T*>(a.out) + token * a.out_stride + (long)head * D + V * lane;
 #pragma unroll
   for (int i = 0; i < V; ++i) dst[i] = from_f<T>(acc[i] * inv);
 }

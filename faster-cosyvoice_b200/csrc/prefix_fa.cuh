@@ -75,22 +75,9 @@ struct SfArgs {
   int* count;
   int list_cap;
   // prefix items: blocks of T * tile_tokens tokens x key heads x parts
-  int prefix_items;
+  int prefix_items, prefix_blocks;
   int none_row;         // a row number behind the own keys' tensor: reads as zeros
 };
-
-// Own keys seen by the token that stands `rel` own positions behind the sequence's first.
-__device__ __forceinline__ int sf_limit(const SpArgs& a, int nk, int rel) {
-  if (a.chunk <= 0) return nk;
-  const long at = (long)a.P + rel;
-  if (at < 0) return 0;
-  long lim;
-  if (a.chunk == 1)
-    lim = (long)rel + 1;
-  else
-    lim = (at / a.chunk + 1) * a.chunk - a.P;
-  return lim < 0 ? 0 : (lim < nk ? static_cast<int>(lim) : nk);
-}
 
 // The list of whole items, longest first: entry = (sequence, block of `block` tokens).  One block
 // of threads; a warp takes a sequence, its lanes the blocks.  Entries are ordered by a counting
@@ -115,7 +102,7 @@ __global__ void __launch_bounds__(1024) sp_list_kernel(const SpArgs a, int block
       s.nk = a.kv_lens ? a.kv_lens[b] : s.nq;
       for (int i = lane; (long)i * block < s.nq; i += 32) {
         const int last = min((long)(i + 1) * block, (long)s.nq) - 1;
-        f(b, i, (sf_limit(a, s.nk, s.nk - s.nq + last) + kSfKeys - 1) / kSfKeys);
+        f(b, i, (sp_limit_at(a, s.nk, s.nk - s.nq + last) + kSfKeys - 1) / kSfKeys);
       }
     }
   };
@@ -180,6 +167,30 @@ __global__ void __launch_bounds__(SpFa<D>::THREADS, 1)
   SfSlot* ring = reinterpret_cast<SfSlot*>(smem + C::OFF_BAR + C::RING_OFF);
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
 
+  int prefix_items = f.prefix_items, prefix_parts = A.prefix_parts, prefix_ctas = gridDim.x;
+  if (A.split.n > 0) {
+    griddep_wait();
+    griddep_launch();
+    // this kernel's share of the SMs follows from the own keys
+    __shared__ unsigned long long units;
+    if (threadIdx.x == 0) units = 0;
+    __syncthreads();
+    long mine = 0;
+    for (int b = threadIdx.x; b < A.B; b += C::THREADS) {
+      const SpSeq s = sp_sequence(A, b, false);
+      mine += ss_count(A, s.nq, s.nk).all(A.Hkv);
+    }
+#pragma unroll
+    for (int w = 16; w > 0; w >>= 1) mine += __shfl_xor_sync(0xffffffffu, mine, w);
+    if (lane == 0) atomicAdd(&units, static_cast<unsigned long long>(mine));
+    __syncthreads();
+    const int pick = sp_pick(A.split, static_cast<long>(units));
+    prefix_parts = A.split.parts[pick];
+    prefix_ctas = A.split.ctas[pick];
+    if (static_cast<int>(blockIdx.x) >= prefix_ctas) return;  // leaves its SM to the own keys
+    prefix_items = f.prefix_blocks * A.Hkv * prefix_parts;
+  }
+
   if (threadIdx.x == 0) {
     for (int i = 0; i < QBUF; ++i) {
       mbar_init(bar(C::bQFull + i), 1);
@@ -218,15 +229,17 @@ __global__ void __launch_bounds__(SpFa<D>::THREADS, 1)
   __syncthreads();
   tc_fence_after();
   const uint32_t tmem = *tmem_slot;
-  griddep_wait();
-  griddep_launch();
+  if (A.split.n == 0) {
+    griddep_wait();
+    griddep_launch();
+  }
 
   if (warp >= C::PRODUCER) {
     if constexpr (T == 3) asm volatile("setmaxnreg.dec.sync.aligned.u32 %0;" ::"n"(kFaRegsProducer));
     if (warp == C::PRODUCER && lane == 0) {
       // ---------------- TMA producer: resolves items, publishes them, loads Q and the key tiles
       const int block = T * f.tile_tokens;
-      const int items = f.list ? min(max(f.count[0], 0), f.list_cap) * A.Hkv : f.prefix_items;
+      const int items = f.list ? min(max(f.count[0], 0), f.list_cap) * A.Hkv : prefix_items;
       int g = 0, i = 0;
       bool ok = true;
       auto take = [&](int now) -> int { return f.list ? atomicAdd(f.count + 1, 1) : now; };
@@ -260,8 +273,8 @@ __global__ void __launch_bounds__(SpFa<D>::THREADS, 1)
           o.own = static_cast<int>(s.base);
           o.part = -1;
         } else {
-          o.part = it % A.prefix_parts;
-          it /= A.prefix_parts;
+          o.part = it % prefix_parts;
+          it /= prefix_parts;
           o.hk = it % A.Hkv;
           const long t0 = (long)(it / A.Hkv) * block;
           const int first = max(0, min(A.N, A.cu[0])), end = max(0, min(A.N, A.cu[A.B]));
@@ -270,7 +283,7 @@ __global__ void __launch_bounds__(SpFa<D>::THREADS, 1)
           o.tok0 = static_cast<int>(lo);
           o.ntok = static_cast<int>(hi - lo);
           int t1;
-          sp_piece((A.P + kSfKeys - 1) / kSfKeys, A.prefix_parts, o.part, o.p0, t1);
+          sp_piece((A.P + kSfKeys - 1) / kSfKeys, prefix_parts, o.part, o.p0, t1);
           o.np = t1 - o.p0;
           o.nk = o.rel = o.own = 0;
         }
@@ -281,7 +294,7 @@ __global__ void __launch_bounds__(SpFa<D>::THREADS, 1)
           if (t < T && r0 < o.ntok) {
             const int last = min(r0 + f.tile_tokens, o.ntok) - 1;
             // at least one tile: a row that sees nothing still has to be written
-            seen[t] = max(1, o.np + (o.part < 0 ? (sf_limit(A, o.nk, o.rel + last) + kSfKeys - 1) / kSfKeys : 0));
+            seen[t] = max(1, o.np + (o.part < 0 ? (sp_limit_at(A, o.nk, o.rel + last) + kSfKeys - 1) / kSfKeys : 0));
           }
           o.n[t] = seen[t];
         }
@@ -295,7 +308,7 @@ __global__ void __launch_bounds__(SpFa<D>::THREADS, 1)
         return true;
       };
       SfSlot o{};
-      for (int it = take(blockIdx.x); it < items && ok; it = take(it + gridDim.x)) {
+      for (int it = take(blockIdx.x); it < items && ok; it = take(it + prefix_ctas)) {
         if (!resolve(it, o)) continue;
         const int qb = i % QBUF;
         if (!publish(o)) { ok = false; break; }
@@ -513,7 +526,7 @@ __global__ void __launch_bounds__(SpFa<D>::THREADS, 1)
       const bool warp_rows = __any_sync(0xffffffffu, row_ok);
       // visible keys, counted from the item's first: the prefix tiles, then the own keys
       const int pre = min(a.np * kSfKeys, A.P - a.p0 * kSfKeys);
-      const int lim = a.part < 0 ? sf_limit(A, a.nk, a.rel + min(tok, a.ntok - 1)) : 0;
+      const int lim = a.part < 0 ? sp_limit_at(A, a.nk, a.rel + min(tok, a.ntok - 1)) : 0;
       const int lmax = __reduce_max_sync(0xffffffffu, lim), lmin = __reduce_min_sync(0xffffffffu, lim);
       float m_ref = -INFINITY;
       float lsum[8] = {0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f, 0.f};

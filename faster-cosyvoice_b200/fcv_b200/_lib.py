@@ -240,7 +240,7 @@ _SIGNATURES = {
     "fcv_hift_forward": (_i, [ctypes.POINTER(HiftWeights), ctypes.POINTER(HiftBatch), _vp, ctypes.c_size_t, _vp]),
     "fcv_qk_norm_rope": (_i, [_vp, _i, _i, _l, _i, _i, _i, _vp, _vp, ctypes.c_float, _vp, _vp, _i, _i, _i, _vp, _vp,
                               _l, _vp, _l, _vp, _l, _vp, _l, _vp]),
-    "fcv_shared_prefix_workspace_bytes": (ctypes.c_size_t, [_i, _i, _i, _i, _i, _i, _i]),
+    "fcv_shared_prefix_workspace_bytes": (ctypes.c_size_t, [_i, _i, _i, _i, _i, _i, _l, _i, _i]),
     "fcv_shared_prefix_attention": (_i, [_vp, _l, _vp, _l, _vp, _l, _l, _vp, _l, _vp, _l, _i, _i, _vp, _vp, _vp, _i,
                                          _i, _i, _i, _i, _i, ctypes.c_float, _vp, _l, _vp, ctypes.c_size_t, _vp]),
 }

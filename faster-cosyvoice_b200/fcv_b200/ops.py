@@ -329,7 +329,7 @@ def shared_prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, p
         if any(_overlap(out, t) for t in (q, k, v, prefix_k, prefix_v)):
             raise ValueError("out must not share memory with the inputs")
     with _on(dev):
-        need = _lib.lib().fcv_shared_prefix_workspace_bytes(N, B, H, Hkv, D, P, dt)
+        need = _lib.lib().fcv_shared_prefix_workspace_bytes(N, B, H, Hkv, D, P, rows, kv_lens is None, dt)
         # a workspace of this call alone, from the allocator that knows streams and graph captures
         ws = q.new_empty(need, dtype=torch.uint8) if need else None
         call("fcv_shared_prefix_attention", q.data_ptr(), q_row, k.data_ptr(), k_row, v.data_ptr(), v_row, rows,

@@ -444,10 +444,10 @@ int fcv_qk_norm_rope(const void* qkv, int dtype, int N, long row_stride, int hea
  * they were.  cu_seqlens that decrease or leave [0, N] give device error 611, own keys outside
  * [0, kv_rows) 612 (the sequence is computed without own keys).  Values must be finite where some
  * query of the same sequence sees them; rows behind a sequence's own keys may hold anything.
- * workspace: fcv_shared_prefix_workspace_bytes() bytes, 16-byte aligned; calls that may overlap
- * need one each. */
+ * workspace: fcv_shared_prefix_workspace_bytes() bytes for the same sizes (packed: kv_base and
+ * kv_lens are null), 16-byte aligned; calls that may overlap need one each. */
 size_t fcv_shared_prefix_workspace_bytes(int N, int B, int heads, int kv_heads, int head_dim, int P,
-                                         int dtype);
+                                         long kv_rows, int packed, int dtype);
 int fcv_shared_prefix_attention(const void* q, long q_stride, const void* k, long k_stride, const void* v,
                                 long v_stride, long kv_rows, const void* prefix_k, long prefix_k_stride,
                                 const void* prefix_v, long prefix_v_stride, int P, int dtype,

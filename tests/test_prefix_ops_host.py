@@ -57,8 +57,8 @@ def test_norm_refuses(lib, bad, status):
     (dict(head_dim=32), -2), (dict(head_dim=256), -2), (dict(q=None), -1), (dict(k=None), -1), (dict(pv=None), -1),
     (dict(cu=None), -1), (dict(out=None), -1), (dict(base=None), -1), (dict(lens=None), -1), (dict(q=A + 2), -1),
     (dict(out=A + 8), -1), (dict(qs=1025), -1), (dict(ks=1025), -1), (dict(pvs=1025), -1), (dict(os=1025), -1),
-    (dict(ws_bytes=16), -1), (dict(scale=0.0), -1), (dict(scale=-0.1), -1),
-    (dict(scale=float("nan")), -1), (dict(scale=float("inf")), -1), (dict(ws=None), -1), (dict(ws=A + 4), -1),
+    (dict(ws_bytes=16, P=100000), -1), (dict(scale=0.0), -1), (dict(scale=-0.1), -1),
+    (dict(scale=float("nan")), -1), (dict(scale=float("inf")), -1), (dict(ws=None, P=100000), -1), (dict(ws=A + 4, P=100000), -1),
 ])
 def test_attention_refuses(lib, bad, status):
     assert attend(lib, **bad) == status
@@ -73,13 +73,13 @@ def test_empty_calls_return_before_any_launch(lib):
 
 def test_workspace_is_sized_on_the_host(lib):
     size = lib.fcv_shared_prefix_workspace_bytes
-    assert size(0, 4, 16, 16, 64, 100, 1) == 0
-    assert size(4, 0, 16, 16, 64, 100, 1) == 0
-    assert size(4, 4, 16, 3, 64, 100, 1) == 0
-    assert size(4, 4, 16, 16, 64, -1, 1) == 0
+    assert size(0, 4, 16, 16, 64, 100, 6400, 0, 1) == 0
+    assert size(4, 0, 16, 16, 64, 100, 6400, 0, 1) == 0
+    assert size(4, 4, 16, 3, 64, 100, 6400, 0, 1) == 0
+    assert size(4, 4, 16, 16, 64, -1, 6400, 0, 1) == 0
     # at least one part of the prefix and one of the own keys: output, maximum and sum of every head
-    assert size(4, 4, 16, 16, 64, 100, 5) == 0
-    assert size(64, 64, 32, 8, 128, 4096, 0) >= 2 * 64 * 32 * (128 * 4 + 8)
+    assert size(4, 4, 16, 16, 64, 100, 6400, 0, 5) == 0
+    assert size(64, 64, 32, 8, 128, 4096, 6400, 0, 0) >= 2 * 64 * 32 * (128 * 4 + 8)
 
 
 def test_cpu_tensors_are_refused():
