@@ -725,7 +725,7 @@ int launch_sp_pieces(const SpArgs& a, dim3 grid, cudaStream_t s) {
   constexpr int R = RP > RO ? RP : RO;
   int smem;
   if constexpr (sizeof(T) == 2) smem = SpMma<D>::kSmem;
-  else smem = SpF32<D, R / 16>::kSmem;
+  else smem = SpF32<D, R / 8>::kSmem;
   static bool attr[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);
@@ -733,7 +733,7 @@ int launch_sp_pieces(const SpArgs& a, dim3 grid, cudaStream_t s) {
     FCV_CUDA(cudaFuncSetAttribute(sp_pieces_kernel<T, D, RP, RO>, cudaFuncAttributeMaxDynamicSharedMemorySize, smem));
     attr[dev & 63] = true;
   }
-  FCV_LAUNCH("sp_pieces_kernel", sp_pieces_kernel<T, D, RP, RO>, grid, dim3(sizeof(T) == 2 ? 128 : 256), smem, s, a);
+  FCV_LAUNCH("sp_pieces_kernel", sp_pieces_kernel<T, D, RP, RO>, grid, dim3(128), smem, s, a);
   return FCV_OK;
 }
 // Own keys of a decode step, streamed (bf16, at most 16 stacked rows of a sequence in a row block).

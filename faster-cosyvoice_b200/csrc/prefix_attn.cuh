@@ -401,12 +401,23 @@ __device__ __forceinline__ void sp_mma_piece(const SpArgs& a, uint8_t* smem, con
 }
 
 // ------------------------------------------------------------------ fp32 (CUDA cores)
-// 256 threads, 16 x 16: thread (ty, tx) has rows RPT ty .. and, of S, keys tx + 16 j, of O,
+// d (two floats) += a b, as one instruction.
+__device__ __forceinline__ void ffma2(float2& d, const float2& a, const float2& b) {
+  asm("{\n\t.reg .b64 a, b, d;\n\t"
+      "mov.b64 a, {%2, %3};\n\tmov.b64 b, {%4, %5};\n\tmov.b64 d, {%0, %1};\n\t"
+      "fma.rn.f32x2 d, a, b, d;\n\tmov.b64 {%0, %1}, d;\n\t}"
+      : "+f"(d.x), "+f"(d.y)
+      : "f"(a.x), "f"(a.y), "f"(b.x), "f"(b.y));
+}
+// 128 threads, 8 x 16: thread (ty, tx) has rows RPT ty .. and, of S, keys tx + 16 j, of O,
 // columns 4 tx + 64 c.  Rows in shared memory are padded by 4 floats, so the 16-byte reads of 8
-// neighbouring rows fall into different banks.
+// neighbouring rows fall into different banks.  Bound by the FMA pipe and, beside it, by the
+// shared-memory reads: with 8 rows a thread, 12 16-byte reads feed 128 multiply-adds; S keeps two
+// partial sums (even and odd d), so that a pair of them is one instruction.
 template <int D, int RPT>
 struct SpF32 {
-  static constexpr int kRows = 16 * RPT;
+  static constexpr int kRows = 8 * RPT;
+  static constexpr int kThreads = 128;
   static constexpr int kLd = D + 4;
   static constexpr int kStages = 2;
   static constexpr int kSmem = 4 * (kRows * kLd + kStages * 2 * kSpKeys * kLd + kRows * (kSpKeys + 4));
@@ -416,7 +427,7 @@ __device__ __forceinline__ void sp_f32_piece(const SpArgs& a, uint8_t* smem, con
                                              const SpKeys<float>& own, int hk, long R0, int rows, int part,
                                              Limit limit) {
   using C = SpF32<D, RPT>;
-  constexpr int LD = C::kLd, CH = D / 4, PLD = kSpKeys + 4;
+  constexpr int LD = C::kLd, CH = D / 4, PLD = kSpKeys + 4, TH = C::kThreads;
   float* sQ = reinterpret_cast<float*>(smem);
   float* sKV = sQ + C::kRows * LD;
   float* sP = sKV + C::kStages * 2 * kSpKeys * LD;
@@ -424,14 +435,14 @@ __device__ __forceinline__ void sp_f32_piece(const SpArgs& a, uint8_t* smem, con
   const bool direct = part < 0;
   const int n_pre = pre.t1 - pre.t0, tiles = n_pre + own.t1 - own.t0;
   __syncthreads();
-  for (int i = tid; i < C::kRows * CH; i += 256) {
+  for (int i = tid; i < C::kRows * CH; i += TH) {
     const int r = i / CH, c = i % CH;
     const bool ok = r < rows;
     const SpRow x = sp_row(a, hk, R0 + (ok ? r : 0));
     cp_async16(smem_u32(sQ + r * LD + 4 * c),
                static_cast<const float*>(a.q) + x.token * a.q_stride + (long)x.head * D + 4 * c, ok);
   }
-  const int lr = tid / CH, lc = tid % CH;  // this thread copies chunk lc of rows lr, lr + 256 / CH, ...
+  const int lr = tid / CH, lc = tid % CH;  // this thread copies chunk lc of rows lr, lr + TH / CH, ...
   auto load = [&](int u) {
     const bool first = u < n_pre;
     const SpKeys<float>& src = first ? pre : own;
@@ -440,9 +451,9 @@ __device__ __forceinline__ void sp_f32_piece(const SpArgs& a, uint8_t* smem, con
     float* vb = kb + kSpKeys * LD;
     const float* kp = src.k + key * src.ks + 4 * lc;
     const float* vp = src.v + key * src.vs + 4 * lc;
-#pragma unroll
-    for (int j = 0; j < kSpKeys * CH / 256; ++j) {
-      constexpr int step = 256 / CH;
+#pragma unroll 4
+    for (int j = 0; j < kSpKeys * CH / TH; ++j) {
+      constexpr int step = TH / CH;
       const bool ok = key + j * step < src.kend;
       cp_async16(smem_u32(kb + j * step * LD), ok ? kp + j * step * src.ks : src.k, ok);
       cp_async16(smem_u32(vb + j * step * LD), ok ? vp + j * step * src.vs : src.v, ok);
@@ -468,10 +479,12 @@ __device__ __forceinline__ void sp_f32_piece(const SpArgs& a, uint8_t* smem, con
     cp_async_commit();
     const float* kb = sKV + (t & 1) * 2 * kSpKeys * LD;
     const float* vb = kb + kSpKeys * LD;
-    float s[RPT][4];
+    float2 s2[RPT][4];
 #pragma unroll
-    for (int i = 0; i < RPT; ++i) s[i][0] = s[i][1] = s[i][2] = s[i][3] = 0.f;
-#pragma unroll 4
+    for (int i = 0; i < RPT; ++i)
+#pragma unroll
+      for (int j = 0; j < 4; ++j) s2[i][j] = make_float2(0.f, 0.f);
+#pragma unroll 2
     for (int d = 0; d < D; d += 4) {
       float4 kv[4];
 #pragma unroll
@@ -481,10 +494,8 @@ __device__ __forceinline__ void sp_f32_piece(const SpArgs& a, uint8_t* smem, con
         const float4 qv = *reinterpret_cast<const float4*>(sQ + (RPT * ty + i) * LD + d);
 #pragma unroll
         for (int j = 0; j < 4; ++j) {
-          s[i][j] = fmaf(qv.x, kv[j].x, s[i][j]);
-          s[i][j] = fmaf(qv.y, kv[j].y, s[i][j]);
-          s[i][j] = fmaf(qv.z, kv[j].z, s[i][j]);
-          s[i][j] = fmaf(qv.w, kv[j].w, s[i][j]);
+          ffma2(s2[i][j], make_float2(qv.x, qv.y), make_float2(kv[j].x, kv[j].y));
+          ffma2(s2[i][j], make_float2(qv.z, qv.w), make_float2(kv[j].z, kv[j].w));
         }
       }
     }
@@ -492,12 +503,12 @@ __device__ __forceinline__ void sp_f32_piece(const SpArgs& a, uint8_t* smem, con
     const int k0 = (first ? pre.t0 + t : own.t0 + t - n_pre) * kSpKeys + tx;
 #pragma unroll
     for (int i = 0; i < RPT; ++i) {
-      float x = -INFINITY;
+      float x = -INFINITY, s[4];
       const int z = first ? pre.kend : lim[i];
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        s[i][j] = k0 + 16 * j < z ? s[i][j] * a.scale_log2 : -INFINITY;
-        x = fmaxf(x, s[i][j]);
+        s[j] = k0 + 16 * j < z ? (s2[i][j].x + s2[i][j].y) * a.scale_log2 : -INFINITY;
+        x = fmaxf(x, s[j]);
       }
 #pragma unroll
       for (int w = 1; w < 16; w <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, w));
@@ -507,7 +518,7 @@ __device__ __forceinline__ void sp_f32_piece(const SpArgs& a, uint8_t* smem, con
       float y = 0.f;
 #pragma unroll
       for (int j = 0; j < 4; ++j) {
-        const float p = exp2f(s[i][j] - ref);
+        const float p = exp2f(s[j] - ref);
         y += p;
         sP[(RPT * ty + i) * PLD + tx + 16 * j] = p;
       }
@@ -584,7 +595,7 @@ __device__ __forceinline__ void sp_block(const SpArgs& a, uint8_t* smem) {
     if constexpr (sizeof(T) == 2)
       sp_mma_piece<D, R / 16>(a, smem, pre, own, hk, R0, rows, part, limit);
     else
-      sp_f32_piece<D, R / 16>(a, smem, pre, own, hk, R0, rows, part, limit);
+      sp_f32_piece<D, R / 8>(a, smem, pre, own, hk, R0, rows, part, limit);
   };
   int it = blockIdx.x;
   SpKeys<T> pre{static_cast<const T*>(a.pk), static_cast<const T*>(a.pv), a.pk_stride, a.pv_stride, a.P, 0, 0};
@@ -629,7 +640,7 @@ __device__ __forceinline__ void sp_block(const SpArgs& a, uint8_t* smem) {
   }
 }
 template <typename T, int D, int RP, int RO>
-__global__ void __launch_bounds__(sizeof(T) == 2 ? 128 : 256) sp_pieces_kernel(const SpArgs a) {
+__global__ void __launch_bounds__(128) sp_pieces_kernel(const SpArgs a) {
   extern __shared__ __align__(128) uint8_t smem[];
   if (!a.beside) griddep_wait();
   griddep_launch();
