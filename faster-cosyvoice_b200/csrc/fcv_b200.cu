@@ -1295,10 +1295,8 @@ int fcv_qk_norm_rope(const void* qkv, int dtype, int N, long row_stride, int hea
   a.v_stride = v_stride;
   a.kv_rows = kv_rows;
   a.kv_limit = kv_limit;
-  // a warp per token once there are enough tokens to fill the GPU; fewer tokens share out their heads
-  const int steps = (heads + (v_out ? 2 : 1) * kv_heads + 256 / head_dim - 1) / (256 / head_dim);
-  const long want = 32L * num_sms();
-  a.warps_per_row = (int)std::max(1L, std::min((long)steps, want / N));
+  const int steps = (heads + kv_heads + 256 / head_dim - 1) / (256 / head_dim);
+  a.warps_per_row = (int)std::max(1L, std::min((long)steps, 8L * num_sms() / N));
   cudaStream_t s = as_stream(stream);
   return dtype == FCV_DTYPE_BF16 ? run_qk_norm<bf16>(a, head_dim, interleaved != 0, s)
                                  : run_qk_norm<float>(a, head_dim, interleaved != 0, s);

@@ -77,91 +77,95 @@ struct Vec8<float> {
 
 // A warp takes (a share of) one token's heads, 256 / D heads at a time: D / 8 lanes hold a head,
 // 8 values each, so loads and stores are 16 bytes wide (32 in float32) and the sum of squares is a
-// few shuffles.  The token's cos / sin values stay in registers over its heads.  Two groups of
-// heads are loaded before either is finished.
+// few shuffles.  The token's cos / sin values and the weights stay in registers over its heads; U
+// steps are loaded before any is finished, the first of them before the token's position is known.
 template <typename T, int D, bool INTERLEAVED>
-__global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QkNormArgs a) {
+__global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) qk_norm_rope_kernel(const QkNormArgs a) {
   griddep_wait();
   griddep_launch();
   constexpr int L = D / 8;          // lanes of a head
   constexpr int HPW = 32 / L;       // heads of one step of the warp
-  constexpr int U = 2;              // steps in flight
+  constexpr int U = sizeof(T) == 2 ? 4 : 2;  // steps in flight
   const int lane = threadIdx.x & 31;
   const long w = (long)blockIdx.x * (blockDim.x >> 5) + (threadIdx.x >> 5);
   const long n = w / a.warps_per_row;
   const int part = static_cast<int>(w - n * a.warps_per_row);
   if (n >= a.N) return;
+  const int sub = lane / L, l = lane % L, d0 = 8 * l;
+  const T* row = static_cast<const T*>(a.qkv) + n * a.row_stride + d0;
+  const int step = HPW * a.warps_per_row;
+  const int units = a.heads + a.kv_heads;
+  Vec8<T> v[U];
+  auto load = [&](int base, int end) {
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = base + u * step + sub;
+      if (h < end) v[u].load(row + (long)h * D);
+    }
+  };
+  load(part * HPW, units);
   const int pos = a.positions[n];
+  long kv_row = a.kv_rows ? a.kv_rows[n] : n;
   if (pos < 0 || pos >= a.rope_rows) {
     if (lane == 0) record_error(601);
     return;
   }
-  long kv_row = a.kv_rows ? a.kv_rows[n] : n;
   if (kv_row >= a.kv_limit) {
     if (lane == 0) record_error(602);
     kv_row = -1;
   }
-  const int sub = lane / L, l = lane % L, d0 = 8 * l;
-  const int units = a.heads + (a.v_out ? 2 : 1) * a.kv_heads;
-  const int qk_units = a.heads + a.kv_heads;
-
-  float wq[8], wk[8], cs[8], sn[8];
-#pragma unroll
-  for (int i = 0; i < 8; ++i) wq[i] = wk[i] = 1.f;
-  Vec8<float> t;
-  if (a.q_weight) t.load(a.q_weight + d0), t.get(wq);
-  if (a.k_weight) t.load(a.k_weight + d0), t.get(wk);
   // rotation of this lane's values: INTERLEAVED uses pairs 4l .. 4l+3 (cs[0..3]); halves use table
   // entries d0 mod half, the partner values sitting half / 8 lanes away
+  float cs[8], sn[8];
   const bool rot = d0 < 2 * a.half;
   int src = lane;
-  float sign = 0.f;
   if (rot) {
-    const long row = (long)pos * a.half;
+    const long at = (long)pos * a.half;
     if (INTERLEAVED) {
-      const float4 c4 = *reinterpret_cast<const float4*>(a.cos + row + 4 * l);
-      const float4 s4 = *reinterpret_cast<const float4*>(a.sin + row + 4 * l);
+      const float4 c4 = *reinterpret_cast<const float4*>(a.cos + at + 4 * l);
+      const float4 s4 = *reinterpret_cast<const float4*>(a.sin + at + 4 * l);
       cs[0] = c4.x, cs[1] = c4.y, cs[2] = c4.z, cs[3] = c4.w;
       sn[0] = s4.x, sn[1] = s4.y, sn[2] = s4.z, sn[3] = s4.w;
     } else {
       const bool low = d0 < a.half;
-      const long i = row + (low ? d0 : d0 - a.half);
+      const long i = at + (low ? d0 : d0 - a.half);
+      Vec8<float> t;
       t.load(a.cos + i), t.get(cs);
       t.load(a.sin + i), t.get(sn);
       src = lane + (low ? a.half / 8 : -a.half / 8);
-      sign = low ? -1.f : 1.f;
+      if (low) {
+#pragma unroll
+        for (int j = 0; j < 8; ++j) sn[j] = -sn[j];
+      }
     }
   }
-  const T* row = static_cast<const T*>(a.qkv) + n * a.row_stride;
-  const int step = HPW * a.warps_per_row;
+  // queries, then keys (a step may hold the last of the one and the first of the other)
   for (int base = part * HPW; base < units; base += U * step) {
-    Vec8<T> v[U];
-#pragma unroll
-    for (int u = 0; u < U; ++u) {
-      const int h = base + u * step + sub;
-      if (h < units) v[u].load(row + (long)h * D + d0);
-    }
+    if (base != part * HPW) load(base, units);
 #pragma unroll
     for (int u = 0; u < U; ++u) {
       const int h0 = base + u * step;
       if (h0 >= units) break;  // warp-uniform
       const int h = h0 + sub;
-      float x[8];
-      if (h < qk_units) {
-        v[u].get(x);
+      const bool is_q = h < a.heads;
+      const float* wp = is_q ? a.q_weight : a.k_weight;
+      float x[8], wt[8];
+      if (wp) {
+        Vec8<float> t;
+        t.load(wp + d0), t.get(wt);
       } else {
 #pragma unroll
-        for (int i = 0; i < 8; ++i) x[i] = 0.f;
+        for (int i = 0; i < 8; ++i) wt[i] = 1.f;
       }
+      v[u].get(x);
       float ss = 0.f;
 #pragma unroll
       for (int i = 0; i < 8; ++i) ss = fmaf(x[i], x[i], ss);
 #pragma unroll
       for (int o = L / 2; o > 0; o >>= 1) ss += __shfl_xor_sync(0xffffffffu, ss, o);
       const float r = rsqrtf(ss * (1.f / D) + a.eps);
-      const bool is_q = h < a.heads;
 #pragma unroll
-      for (int i = 0; i < 8; ++i) x[i] = x[i] * r * (is_q ? wq[i] : wk[i]);
+      for (int i = 0; i < 8; ++i) x[i] = x[i] * r * wt[i];
       if (INTERLEAVED) {
         if (rot) {
 #pragma unroll
@@ -175,18 +179,24 @@ __global__ void __launch_bounds__(256) qk_norm_rope_kernel(const QkNormArgs a) {
 #pragma unroll
         for (int i = 0; i < 8; ++i) {
           const float other = __shfl_sync(0xffffffffu, x[i], src);
-          if (rot) x[i] = x[i] * cs[i] + sign * other * sn[i];
+          if (rot) x[i] = x[i] * cs[i] + other * sn[i];
         }
       }
-      if (h < qk_units) v[u].set(x);
-      if (is_q) {
+      v[u].set(x);
+      if (is_q)
         v[u].store(static_cast<T*>(a.q_out) + n * a.q_stride + (long)h * D + d0);
-      } else if (h < units && kv_row >= 0) {
-        if (h < qk_units)
-          v[u].store(static_cast<T*>(a.k_out) + kv_row * a.k_stride + (long)(h - a.heads) * D + d0);
-        else
-          v[u].store(static_cast<T*>(a.v_out) + kv_row * a.v_stride + (long)(h - qk_units) * D + d0);
-      }
+      else if (h < units && kv_row >= 0)
+        v[u].store(static_cast<T*>(a.k_out) + kv_row * a.k_stride + (long)(h - a.heads) * D + d0);
+    }
+  }
+  if (a.v_out == nullptr || kv_row < 0) return;
+  row += (long)units * D;
+  for (int base = part * HPW; base < a.kv_heads; base += U * step) {
+    load(base, a.kv_heads);
+#pragma unroll
+    for (int u = 0; u < U; ++u) {
+      const int h = base + u * step + sub;
+      if (h < a.kv_heads) v[u].store(static_cast<T*>(a.v_out) + kv_row * a.v_stride + (long)h * D + d0);
     }
   }
 }
