@@ -531,7 +531,10 @@ struct SpPlan {
 // of each of 4 streams behind 200 keys (16/16 heads) 13.4 / 7.4 / 15.7; behind 8000 keys 112 / 60 / 29;
 // 32 sequences of about 170 queries behind 2000 keys (32/8 heads) 256 / 688 / 396.
 // The own keys' lengths are on the device: a cache is taken to be half full.
-SpPlan sp_plan(long N, int B, int H, int Hkv, int D, long P, bool bf, long kv_rows, bool packed) {
+SpPlan sp_plan(const fcv_prefix_attention& g) {
+  const long N = g.N, P = g.P, kv_rows = g.kv_rows;
+  const int B = g.B, H = g.heads, Hkv = g.kv_heads, D = g.head_dim;
+  const bool bf = g.dtype == FCV_DTYPE_BF16, packed = g.kv_lens == nullptr;
   SpPlan p{};
   const long G = H / Hkv, q_len = (N + B - 1) / B;
   const long rows = N * G, own = q_len * G;  // stacked rows, and of a sequence
@@ -594,37 +597,36 @@ SpPlan sp_plan(long N, int B, int H, int Hkv, int D, long P, bool bf, long kv_ro
     p.split.sms = (int)sms;
     p.split.unit_us = D == 64 ? 0.33f : 0.66f;
     p.split.floor_us = D == 64 ? 0.0028f : 0.0056f;
-    // candidates: n parts dealt in w even waves; kept where more blocks make the prefix a tenth faster
-    struct Choice {
-      int ctas, parts;
-      float us;
-    };
-    std::vector<Choice> all;
+    // the fastest number of parts for every number of blocks that deals them in even waves; kept
+    // where more blocks make the prefix faster by a tenth or so
+    constexpr int kMost = 256;
+    const int top = (int)std::min(sms, (long)kMost);
+    float us[kMost + 1];
+    int parts[kMost + 1];
+    std::fill(us, us + top + 1, 0.f);
     const long items1 = p.prefix_blocks * Hkv;
+    auto offer = [&](long c, int n, float t) {
+      if (c > top || (us[c] != 0.f && us[c] <= t)) return;
+      us[c] = t;
+      parts[c] = n;
+    };
     for (int n = 1; n <= 24 && (n == 1 || (n - 1) * 4 < tiles); ++n) {
-      const float item = (tiles + n - 1) / n * step_us + item_us;
-      for (int w = 1; w <= 8; ++w) {
-        const long c = (items1 * n + w - 1) / w;
-        if (c <= sms) all.push_back({(int)c, n, w * item + n * 0.1f});
-      }
-      const long w = (items1 * n + sms - 1) / sms;
-      all.push_back({(int)sms, n, w * item + n * 0.1f});
+      const float item = (float)((tiles + n - 1) / n) * step_us + item_us;
+      const long all_items = items1 * n;
+      for (int w = 1; w <= 8; ++w) offer((all_items + w - 1) / w, n, w * item + n * 0.1f);
+      offer(top, n, (float)((all_items + top - 1) / top) * item + n * 0.1f);
     }
-    std::sort(all.begin(), all.end(), [](const Choice& x, const Choice& y) {
-      return x.ctas != y.ctas ? x.ctas < y.ctas : x.us < y.us;
-    });
-    for (float keep = 0.93f;; keep -= 0.05f) {
+    for (float keep = 0.93f; keep > 0.4f; keep -= 0.08f) {
       int n = 0;
       float last = 0.f;
-      for (const Choice& c : all) {
-        if (n > 0 && c.us > keep * last) continue;
-        if (n > 0 && p.split.ctas[n - 1] == c.ctas) continue;
-        if (n < kSplits) p.split.ctas[n] = c.ctas, p.split.parts[n] = c.parts, p.split.fa_us[n] = c.us;
-        last = c.us;
+      for (int c = 1; c <= top && n <= kSplits; ++c) {
+        if (us[c] == 0.f || (n > 0 && us[c] > keep * last)) continue;
+        if (n < kSplits) p.split.ctas[n] = c, p.split.parts[n] = parts[c], p.split.fa_us[n] = us[c];
+        last = us[c];
         ++n;
       }
       p.split.n = std::min(n, kSplits);
-      if (n <= kSplits || keep < 0.5f) break;
+      if (n <= kSplits) break;
     }
     for (int i = 0; i < p.split.n; ++i) p.prefix_parts = std::max(p.prefix_parts, p.split.parts[i]);
     p.fa_ctas = (int)sms;
@@ -1248,123 +1250,124 @@ int fcv_attention(const void* qkv, int dtype, const int32_t* cu_seqlens, int B, 
                        sched_ctas);
 }
 
-int fcv_qk_norm_rope(const void* qkv, int dtype, int N, long row_stride, int heads, int kv_heads, int head_dim,
-                     const float* q_weight, const float* k_weight, float eps, const float* rope_cos,
-                     const float* rope_sin, int rope_rows, int rope_half, int interleaved, const int32_t* positions,
-                     void* q_out, long q_stride, void* k_out, long k_stride, void* v_out, long v_stride,
-                     const int32_t* kv_rows, long kv_limit, void* stream) {
-  if (!valid_dtype(dtype)) return fail(FCV_EINVAL, "fcv_qk_norm_rope: bad dtype");
-  if (N < 0 || heads < 1 || kv_heads < 1 || !(eps >= 0.f) || rope_rows < 0 || kv_limit < 0)
+int fcv_qk_norm_rope(const fcv_qk_norm* g, void* stream) {
+  if (!g) return fail(FCV_EINVAL, "fcv_qk_norm_rope: null arguments");
+  if (!valid_dtype(g->dtype)) return fail(FCV_EINVAL, "fcv_qk_norm_rope: bad dtype");
+  if (g->N < 0 || g->heads < 1 || g->kv_heads < 1 || !(g->eps >= 0.f) || g->rope_rows < 0 || g->kv_limit < 0)
     return fail(FCV_EINVAL, "fcv_qk_norm_rope: bad arguments");
-  if (head_dim != 32 && head_dim != 64 && head_dim != 128 && head_dim != 256)
-    return fail(FCV_EUNSUPPORTED, "fcv_qk_norm_rope: head_dim must be 32, 64, 128 or 256 (got %d)", head_dim);
-  if (rope_half < 8 || rope_half % 8 != 0 || 2 * rope_half > head_dim)
+  if (g->head_dim != 32 && g->head_dim != 64 && g->head_dim != 128 && g->head_dim != 256)
+    return fail(FCV_EUNSUPPORTED, "fcv_qk_norm_rope: head_dim must be 32, 64, 128 or 256 (got %d)", g->head_dim);
+  if (g->rope_half < 8 || g->rope_half % 8 != 0 || 2 * g->rope_half > g->head_dim)
     return fail(FCV_EUNSUPPORTED, "fcv_qk_norm_rope: the rotated width 2 * %d must be a multiple of 16 of at most "
-                "head_dim", rope_half);
-  if (N == 0) return FCV_OK;
-  if (!qkv || !rope_cos || !rope_sin || !positions || !q_out || !k_out)
+                "head_dim", g->rope_half);
+  if (g->N == 0) return FCV_OK;
+  if (!g->qkv || !g->rope_cos || !g->rope_sin || !g->positions || !g->q_out || !g->k_out)
     return fail(FCV_EINVAL, "fcv_qk_norm_rope: null pointer");
-  const long es = (long)dsize(dtype);
-  const uintptr_t at = reinterpret_cast<uintptr_t>(qkv) | reinterpret_cast<uintptr_t>(q_out) |
-                       reinterpret_cast<uintptr_t>(k_out) | reinterpret_cast<uintptr_t>(v_out) |
-                       reinterpret_cast<uintptr_t>(rope_cos) | reinterpret_cast<uintptr_t>(rope_sin) |
-                       reinterpret_cast<uintptr_t>(q_weight) | reinterpret_cast<uintptr_t>(k_weight);
-  if ((at & 15) || ((row_stride * es) & 15) || ((q_stride * es) & 15) || ((k_stride * es) & 15) ||
-      ((v_stride * es) & 15))
+  const long es = (long)dsize(g->dtype);
+  const uintptr_t at = reinterpret_cast<uintptr_t>(g->qkv) | reinterpret_cast<uintptr_t>(g->q_out) |
+                       reinterpret_cast<uintptr_t>(g->k_out) | reinterpret_cast<uintptr_t>(g->v_out) |
+                       reinterpret_cast<uintptr_t>(g->rope_cos) | reinterpret_cast<uintptr_t>(g->rope_sin) |
+                       reinterpret_cast<uintptr_t>(g->q_weight) | reinterpret_cast<uintptr_t>(g->k_weight);
+  if ((at & 15) || (((g->row_stride | g->q_stride | g->k_stride | g->v_stride) * es) & 15))
     return fail(FCV_EINVAL, "fcv_qk_norm_rope: rows, weights and tables must be 16-byte aligned");
-  if (!kv_rows && kv_limit < N) return fail(FCV_EINVAL, "fcv_qk_norm_rope: %d rows into %ld", N, kv_limit);
+  if (!g->kv_rows && g->kv_limit < g->N)
+    return fail(FCV_EINVAL, "fcv_qk_norm_rope: %d rows into %ld", g->N, g->kv_limit);
   QkNormArgs a{};
-  a.qkv = qkv;
-  a.row_stride = row_stride;
-  a.N = N;
-  a.heads = heads;
-  a.kv_heads = kv_heads;
-  a.q_weight = q_weight;
-  a.k_weight = k_weight;
-  a.eps = eps;
-  a.cos = rope_cos;
-  a.sin = rope_sin;
-  a.rope_rows = rope_rows;
-  a.half = rope_half;
-  a.positions = positions;
-  a.q_out = q_out;
-  a.q_stride = q_stride;
-  a.k_out = k_out;
-  a.k_stride = k_stride;
-  a.v_out = v_out;
-  a.v_stride = v_stride;
-  a.kv_rows = kv_rows;
-  a.kv_limit = kv_limit;
-  const int steps = (heads + kv_heads + 256 / head_dim - 1) / (256 / head_dim);
-  a.warps_per_row = (int)std::max(1L, std::min((long)steps, 8L * num_sms() / N));
+  a.qkv = g->qkv;
+  a.row_stride = g->row_stride;
+  a.N = g->N;
+  a.heads = g->heads;
+  a.kv_heads = g->kv_heads;
+  a.q_weight = g->q_weight;
+  a.k_weight = g->k_weight;
+  a.eps = g->eps;
+  a.cos = g->rope_cos;
+  a.sin = g->rope_sin;
+  a.rope_rows = g->rope_rows;
+  a.half = g->rope_half;
+  a.positions = g->positions;
+  a.q_out = g->q_out;
+  a.q_stride = g->q_stride;
+  a.k_out = g->k_out;
+  a.k_stride = g->k_stride;
+  a.v_out = g->v_out;
+  a.v_stride = g->v_stride;
+  a.kv_rows = g->kv_rows;
+  a.kv_limit = g->kv_limit;
+  // A warp per token; tokens too few to give every SM eight warps share out their heads (one token of
+  // 16/16 heads of 64: 2.2 us against 3.6).  More warps per token cost more than they hide: each reads
+  // the position, the tables and the weights again (96000 tokens: 1, 2, 3 warps 144, 156, 190 us).
+  const int steps = (g->heads + g->kv_heads + 256 / g->head_dim - 1) / (256 / g->head_dim);
+  a.warps_per_row = (int)std::max(1L, std::min((long)steps, 8L * num_sms() / g->N));
   cudaStream_t s = as_stream(stream);
-  return dtype == FCV_DTYPE_BF16 ? run_qk_norm<bf16>(a, head_dim, interleaved != 0, s)
-                                 : run_qk_norm<float>(a, head_dim, interleaved != 0, s);
+  return g->dtype == FCV_DTYPE_BF16 ? run_qk_norm<bf16>(a, g->head_dim, g->interleaved != 0, s)
+                                    : run_qk_norm<float>(a, g->head_dim, g->interleaved != 0, s);
 }
 
-size_t fcv_shared_prefix_workspace_bytes(int N, int B, int heads, int kv_heads, int head_dim, int P, long kv_rows,
-                                         int packed, int dtype) {
-  if (!valid_dtype(dtype) || kv_rows < 0 || N <= 0 || B <= 0 || heads < 1 || kv_heads < 1 || heads % kv_heads != 0 || P < 0) return 0;
-  return sp_plan(N, B, heads, kv_heads, head_dim, P, dtype == FCV_DTYPE_BF16, kv_rows, packed != 0).bytes;
+size_t fcv_shared_prefix_workspace_bytes(const fcv_prefix_attention* g) {
+  if (!g || !valid_dtype(g->dtype) || g->kv_rows < 0 || g->N <= 0 || g->B <= 0 || g->heads < 1 || g->kv_heads < 1 ||
+      g->heads % g->kv_heads != 0 || g->P < 0 || (g->head_dim != 64 && g->head_dim != 128))
+    return 0;
+  return sp_plan(*g).bytes;
 }
 
-int fcv_shared_prefix_attention(const void* q, long q_stride, const void* k, long k_stride, const void* v,
-                                long v_stride, long kv_rows, const void* prefix_k, long prefix_k_stride,
-                                const void* prefix_v, long prefix_v_stride, int P, int dtype,
-                                const int32_t* cu_seqlens, const int32_t* kv_base, const int32_t* kv_lens, int B,
-                                int N, int heads, int kv_heads, int head_dim, int chunk, float scale, void* out,
-                                long out_stride, void* workspace, size_t workspace_bytes, void* stream) {
-  if (!valid_dtype(dtype)) return fail(FCV_EINVAL, "fcv_shared_prefix_attention: bad dtype");
-  if (B < 0 || N < 0 || P < 0 || kv_rows < 0 || chunk < 0 || heads < 1 || kv_heads < 1)
+int fcv_shared_prefix_attention(const fcv_prefix_attention* g, void* workspace, size_t workspace_bytes, void* stream) {
+  if (!g) return fail(FCV_EINVAL, "fcv_shared_prefix_attention: null arguments");
+  if (!valid_dtype(g->dtype)) return fail(FCV_EINVAL, "fcv_shared_prefix_attention: bad dtype");
+  const int B = g->B, N = g->N, P = g->P, heads = g->heads, kv_heads = g->kv_heads, head_dim = g->head_dim;
+  const long kv_rows = g->kv_rows;
+  if (B < 0 || N < 0 || P < 0 || kv_rows < 0 || g->chunk < 0 || heads < 1 || kv_heads < 1)
     return fail(FCV_EINVAL, "fcv_shared_prefix_attention: bad arguments");
   if (heads % kv_heads != 0)
     return fail(FCV_EINVAL, "fcv_shared_prefix_attention: %d heads over %d key heads", heads, kv_heads);
   if (head_dim != 64 && head_dim != 128)
     return fail(FCV_EUNSUPPORTED, "fcv_shared_prefix_attention: head_dim must be 64 or 128 (got %d)", head_dim);
-  if (!(scale > 0.f) || scale > 3.0e38f) return fail(FCV_EINVAL, "fcv_shared_prefix_attention: scale must be positive");
+  if (!(g->scale > 0.f) || g->scale > 3.0e38f)
+    return fail(FCV_EINVAL, "fcv_shared_prefix_attention: scale must be positive");
   if (N == 0 || B == 0) return FCV_OK;
-  if (!q || !cu_seqlens || !out || (kv_rows > 0 && (!k || !v)) || (P > 0 && (!prefix_k || !prefix_v)) ||
-      (!kv_base != !kv_lens))
+  if (!g->q || !g->cu_seqlens || !g->out || (kv_rows > 0 && (!g->k || !g->v)) ||
+      (P > 0 && (!g->prefix_k || !g->prefix_v)) || (!g->kv_base != !g->kv_lens))
     return fail(FCV_EINVAL, "fcv_shared_prefix_attention: null pointer");
-  const long es = (long)dsize(dtype);
-  const uintptr_t at = reinterpret_cast<uintptr_t>(q) | reinterpret_cast<uintptr_t>(k) |
-                       reinterpret_cast<uintptr_t>(v) | reinterpret_cast<uintptr_t>(prefix_k) |
-                       reinterpret_cast<uintptr_t>(prefix_v) | reinterpret_cast<uintptr_t>(out);
-  if ((at & 15) || ((q_stride * es) & 15) || ((k_stride * es) & 15) || ((v_stride * es) & 15) ||
-      ((prefix_k_stride * es) & 15) || ((prefix_v_stride * es) & 15) || ((out_stride * es) & 15))
+  const long es = (long)dsize(g->dtype);
+  const uintptr_t at = reinterpret_cast<uintptr_t>(g->q) | reinterpret_cast<uintptr_t>(g->k) |
+                       reinterpret_cast<uintptr_t>(g->v) | reinterpret_cast<uintptr_t>(g->prefix_k) |
+                       reinterpret_cast<uintptr_t>(g->prefix_v) | reinterpret_cast<uintptr_t>(g->out);
+  const long strides = g->q_stride | g->k_stride | g->v_stride | g->prefix_k_stride | g->prefix_v_stride |
+                       g->out_stride;
+  if ((at & 15) || ((strides * es) & 15))
     return fail(FCV_EINVAL, "fcv_shared_prefix_attention: rows must be 16-byte aligned");
   if (P > 0x7fffff00 || kv_rows > 0x7fffff00L)  // row numbers of a tile past the last row stay 32-bit
     return fail(FCV_EUNSUPPORTED, "fcv_shared_prefix_attention: too many key rows");
-  SpPlan p = sp_plan(N, B, heads, kv_heads, head_dim, P, dtype == FCV_DTYPE_BF16, kv_rows, !kv_lens);
+  SpPlan p = sp_plan(*g);
   if (workspace_bytes < p.bytes || (p.bytes && !workspace) || (reinterpret_cast<uintptr_t>(workspace) & 15))
     return fail(FCV_EINVAL, "fcv_shared_prefix_attention: workspace of %zu bytes, %zu needed", workspace_bytes, p.bytes);
   if (p.prefix_blocks * kv_heads * p.prefix_parts > 0x7fffffffL)
     return fail(FCV_EUNSUPPORTED, "fcv_shared_prefix_attention: too many blocks");
   SpArgs a{};
-  a.q = q;
-  a.q_stride = q_stride;
-  a.k = k;
-  a.v = v;
-  a.k_stride = k_stride;
-  a.v_stride = v_stride;
+  a.q = g->q;
+  a.q_stride = g->q_stride;
+  a.k = g->k;
+  a.v = g->v;
+  a.k_stride = g->k_stride;
+  a.v_stride = g->v_stride;
   a.kv_rows = kv_rows;
-  a.pk = prefix_k;
-  a.pv = prefix_v;
-  a.pk_stride = prefix_k_stride;
-  a.pv_stride = prefix_v_stride;
+  a.pk = g->prefix_k;
+  a.pv = g->prefix_v;
+  a.pk_stride = g->prefix_k_stride;
+  a.pv_stride = g->prefix_v_stride;
   a.P = P;
-  a.cu = cu_seqlens;
-  a.kv_base = kv_base;
-  a.kv_lens = kv_lens;
+  a.cu = g->cu_seqlens;
+  a.kv_base = g->kv_base;
+  a.kv_lens = g->kv_lens;
   a.B = B;
   a.N = N;
   a.H = heads;
   a.Hkv = kv_heads;
   a.G = heads / kv_heads;
-  a.chunk = chunk;
-  a.scale_log2 = scale * kLog2e;
-  a.out = out;
-  a.out_stride = out_stride;
+  a.chunk = g->chunk;
+  a.scale_log2 = g->scale * kLog2e;
+  a.out = g->out;
+  a.out_stride = g->out_stride;
   a.prefix_parts = p.prefix_parts;
   a.own_parts = p.own_parts;
   a.whole = p.whole ? 1 : 0;
@@ -1416,7 +1419,7 @@ int fcv_shared_prefix_attention(const void* q, long q_stride, const void* k, lon
   }
   a.part_o = static_cast<float*>(workspace);
   a.part_ml = reinterpret_cast<float2*>(static_cast<float*>(workspace) + rows * head_dim);
-  if (dtype == FCV_DTYPE_BF16)
+  if (g->dtype == FCV_DTYPE_BF16)
     return head_dim == 64 ? run_sp<bf16, 64>(a, p, s) : run_sp<bf16, 128>(a, p, s);
   return head_dim == 64 ? run_sp<float, 64>(a, p, s) : run_sp<float, 128>(a, p, s);
 }

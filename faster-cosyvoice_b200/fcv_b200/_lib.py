@@ -9,6 +9,7 @@ from __future__ import annotations
 
 import ctypes
 import os
+import struct
 import threading
 
 _HERE = os.path.dirname(os.path.abspath(__file__))
@@ -198,6 +199,11 @@ class HiftBatch(ctypes.Structure):
     ]
 
 
+# Argument structures that are filled on every call of a short operator: packing them takes a fraction
+# of the time that ctypes needs for as many arguments.  The layouts are those of the header's structures.
+QK_NORM = struct.Struct("@10P5l8if4x")  # fcv_qk_norm
+PREFIX_ATTENTION = struct.Struct("@9P7l8if4x")  # fcv_prefix_attention
+
 _lock = threading.Lock()
 _lib = None
 
@@ -238,11 +244,9 @@ _SIGNATURES = {
     "fcv_pack_rows": (_i, [_vp, _i, _l, _i, _vp, _i, _i, _vp, _i, _vp]),
     "fcv_hift_workspace_bytes": (ctypes.c_size_t, [ctypes.POINTER(ctypes.c_int)]),
     "fcv_hift_forward": (_i, [ctypes.POINTER(HiftWeights), ctypes.POINTER(HiftBatch), _vp, ctypes.c_size_t, _vp]),
-    "fcv_qk_norm_rope": (_i, [_vp, _i, _i, _l, _i, _i, _i, _vp, _vp, ctypes.c_float, _vp, _vp, _i, _i, _i, _vp, _vp,
-                              _l, _vp, _l, _vp, _l, _vp, _l, _vp]),
-    "fcv_shared_prefix_workspace_bytes": (ctypes.c_size_t, [_i, _i, _i, _i, _i, _i, _l, _i, _i]),
-    "fcv_shared_prefix_attention": (_i, [_vp, _l, _vp, _l, _vp, _l, _l, _vp, _l, _vp, _l, _i, _i, _vp, _vp, _vp, _i,
-                                         _i, _i, _i, _i, _i, ctypes.c_float, _vp, _l, _vp, ctypes.c_size_t, _vp]),
+    "fcv_qk_norm_rope": (_i, [_vp, _vp]),
+    "fcv_shared_prefix_workspace_bytes": (ctypes.c_size_t, [_vp]),
+    "fcv_shared_prefix_attention": (_i, [_vp, _vp, ctypes.c_size_t, _vp]),
 }
 
 

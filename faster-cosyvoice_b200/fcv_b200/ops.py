@@ -240,7 +240,7 @@ def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: tor
         q, q_row = qkv.as_strided((N, heads, D), (row, D, 1)), row
     else:
         q, q_row = qkv.new_empty((N, heads, D)), q_width
-    v_ptr = rows_ptr = None
+    v_ptr = rows_ptr = 0
     if kv_cache is not None:
         _int32("kv_rows", kv_rows, N)
         if kv_cache.dim() != 2 or kv_cache.shape[1] != 2 * k_width or kv_cache.dtype is not qkv.dtype:
@@ -260,11 +260,12 @@ def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: tor
     else:
         second = qkv.new_empty((N, kv_heads, D))
         k_ptr, k_row, limit = second.data_ptr(), k_width, N
+    args = _lib.QK_NORM.pack(
+        ptr, 0 if q_weight is None else q_weight.data_ptr(), 0 if k_weight is None else k_weight.data_ptr(),
+        rope_cos.data_ptr(), rope_sin.data_ptr(), positions.data_ptr(), q.data_ptr(), k_ptr, v_ptr, rows_ptr, row,
+        q_row, k_row, k_row, limit, dt, N, heads, kv_heads, D, table[0], table[1], interleaved, eps)
     with _on(dev):
-        call("fcv_qk_norm_rope", ptr, dt, N, row, heads, kv_heads, D, None if q_weight is None else
-             q_weight.data_ptr(), None if k_weight is None else k_weight.data_ptr(), eps, rope_cos.data_ptr(),
-             rope_sin.data_ptr(), table[0], table[1], interleaved, positions.data_ptr(), q.data_ptr(), q_row, k_ptr,
-             k_row, v_ptr, k_row, rows_ptr, limit, _raw_stream(dev))
+        call("fcv_qk_norm_rope", args, _raw_stream(dev))
     return q, second
 
 
@@ -309,7 +310,7 @@ def shared_prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, p
     if B < 0:
         raise ValueError("cu_seqlens must hold at least one entry")
     _int32("cu_seqlens", cu_seqlens, B + 1)
-    base_ptr = lens_ptr = None
+    base_ptr = lens_ptr = 0
     if kv_base is not None and kv_lens is not None:
         _int32("kv_base", kv_base, B)
         _int32("kv_lens", kv_lens, B)
@@ -328,14 +329,15 @@ def shared_prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, p
             raise ValueError("out must be (N, heads, head_dim) rows that do not overlap")
         if any(_overlap(out, t) for t in (q, k, v, prefix_k, prefix_v)):
             raise ValueError("out must not share memory with the inputs")
+    args = _lib.PREFIX_ATTENTION.pack(
+        q.data_ptr(), k.data_ptr(), v.data_ptr(), prefix_k.data_ptr(), prefix_v.data_ptr(), cu_seqlens.data_ptr(),
+        base_ptr, lens_ptr, out.data_ptr(), q_row, k_row, v_row, rows, pk_row, pv_row, out_row, P, dt, B, N, H, Hkv, D,
+        chunk, scale)
     with _on(dev):
-        need = _lib.lib().fcv_shared_prefix_workspace_bytes(N, B, H, Hkv, D, P, rows, kv_lens is None, dt)
+        need = _lib.lib().fcv_shared_prefix_workspace_bytes(args)
         # a workspace of this call alone, from the allocator that knows streams and graph captures
         ws = q.new_empty(need, dtype=torch.uint8) if need else None
-        call("fcv_shared_prefix_attention", q.data_ptr(), q_row, k.data_ptr(), k_row, v.data_ptr(), v_row, rows,
-             prefix_k.data_ptr(), pk_row, prefix_v.data_ptr(), pv_row, P, dt, cu_seqlens.data_ptr(), base_ptr,
-             lens_ptr, B, N, H, Hkv, D, chunk, scale, out.data_ptr(), out_row,
-             None if ws is None else ws.data_ptr(), need, _raw_stream(dev))
+        call("fcv_shared_prefix_attention", args, None if ws is None else ws.data_ptr(), need, _raw_stream(dev))
     return out
 
 

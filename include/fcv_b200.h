@@ -423,11 +423,22 @@ int fcv_pack_rows(const void* src, int src_dtype, long batch_stride, int T, cons
  * unwritten with device error 601, a row >= kv_limit its keys and values with 602.
  * head_dim 32, 64, 128 or 256; rope_half a multiple of 8; all rows, weights and tables 16-byte
  * aligned. */
-int fcv_qk_norm_rope(const void* qkv, int dtype, int N, long row_stride, int heads, int kv_heads, int head_dim,
-                     const float* q_weight, const float* k_weight, float eps, const float* rope_cos,
-                     const float* rope_sin, int rope_rows, int rope_half, int interleaved, const int32_t* positions,
-                     void* q_out, long q_stride, void* k_out, long k_stride, void* v_out, long v_stride,
-                     const int32_t* kv_rows, long kv_limit, void* stream);
+typedef struct fcv_qk_norm {
+  const void* qkv;
+  const float* q_weight;
+  const float* k_weight;
+  const float* rope_cos;
+  const float* rope_sin;
+  const int32_t* positions;
+  void* q_out;
+  void* k_out;
+  void* v_out;
+  const int32_t* kv_rows;
+  long row_stride, q_stride, k_stride, v_stride, kv_limit;
+  int dtype, N, heads, kv_heads, head_dim, rope_rows, rope_half, interleaved;
+  float eps;
+} fcv_qk_norm;
+int fcv_qk_norm_rope(const fcv_qk_norm* args, void* stream);
 
 /* ------------------------------------------------------------------ shared-prefix attention
  * Attention of a ragged batch whose sequences share one prefix of P keys and values (streams of one
@@ -444,16 +455,25 @@ int fcv_qk_norm_rope(const void* qkv, int dtype, int N, long row_stride, int hea
  * they were.  cu_seqlens that decrease or leave [0, N] give device error 611, own keys outside
  * [0, kv_rows) 612 (the sequence is computed without own keys).  Values must be finite where some
  * query of the same sequence sees them; rows behind a sequence's own keys may hold anything.
- * workspace: fcv_shared_prefix_workspace_bytes() bytes for the same sizes (packed: kv_base and
- * kv_lens are null), 16-byte aligned; calls that may overlap need one each. */
-size_t fcv_shared_prefix_workspace_bytes(int N, int B, int heads, int kv_heads, int head_dim, int P,
-                                         long kv_rows, int packed, int dtype);
-int fcv_shared_prefix_attention(const void* q, long q_stride, const void* k, long k_stride, const void* v,
-                                long v_stride, long kv_rows, const void* prefix_k, long prefix_k_stride,
-                                const void* prefix_v, long prefix_v_stride, int P, int dtype,
-                                const int32_t* cu_seqlens, const int32_t* kv_base, const int32_t* kv_lens, int B,
-                                int N, int heads, int kv_heads, int head_dim, int chunk, float scale, void* out,
-                                long out_stride, void* workspace, size_t workspace_bytes, void* stream);
+ * workspace: fcv_shared_prefix_workspace_bytes() bytes for the same arguments (0 for arguments that
+ * are refused), 16-byte aligned; calls that may overlap need one each. */
+typedef struct fcv_prefix_attention {
+  const void* q;
+  const void* k;
+  const void* v;
+  const void* prefix_k;
+  const void* prefix_v;
+  const int32_t* cu_seqlens;
+  const int32_t* kv_base;
+  const int32_t* kv_lens;
+  void* out;
+  long q_stride, k_stride, v_stride, kv_rows, prefix_k_stride, prefix_v_stride, out_stride;
+  int P, dtype, B, N, heads, kv_heads, head_dim, chunk;
+  float scale;
+} fcv_prefix_attention;
+size_t fcv_shared_prefix_workspace_bytes(const fcv_prefix_attention* args);
+int fcv_shared_prefix_attention(const fcv_prefix_attention* args, void* workspace, size_t workspace_bytes,
+                                void* stream);
 
 /* ------------------------------------------------------------------ HiFT vocoder
  * CausalHiFTGenerator (cosyvoice/hifigan/generator.py:578-740) as built by

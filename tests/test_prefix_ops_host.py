@@ -3,9 +3,12 @@ status and a message before any CUDA call, and the workspace is sized by the hos
 
 from __future__ import annotations
 
+import re
+import struct
+
 import pytest
 
-from conftest import ensure_built
+from conftest import ROOT, ensure_built
 
 A = 0x10000  # a 16-byte aligned address; the calls below return before anything is read
 
@@ -19,31 +22,32 @@ def lib():
 
 
 def norm(lib, **kw):
-    a = dict(qkv=A, dtype=1, N=4, stride=3072, heads=16, kv_heads=16, head_dim=64, qw=A, kw=A, eps=1e-6, cos=A, sin=A,
-             rows=128, half=32, inter=1, pos=A, q=A, qs=1024, k=A, ks=1024, v=None, vs=1024, kv_rows=None, limit=4)
+    from fcv_b200 import _lib
+
+    a = dict(qkv=A, qw=A, kw=A, cos=A, sin=A, pos=A, q=A, k=A, v=0, kv_rows=0, stride=3072, qs=1024, ks=1024, vs=1024,
+             limit=4, dtype=1, N=4, heads=16, kv_heads=16, head_dim=64, rows=128, half=32, inter=1, eps=1e-6)
     a.update(kw)
-    return lib.fcv_qk_norm_rope(a["qkv"], a["dtype"], a["N"], a["stride"], a["heads"], a["kv_heads"], a["head_dim"],
-                                a["qw"], a["kw"], a["eps"], a["cos"], a["sin"], a["rows"], a["half"], a["inter"],
-                                a["pos"], a["q"], a["qs"], a["k"], a["ks"], a["v"], a["vs"], a["kv_rows"], a["limit"],
-                                None)
+    return lib.fcv_qk_norm_rope(_lib.QK_NORM.pack(*a.values()), None)
 
 
-def attend(lib, **kw):
-    a = dict(q=A, qs=1024, k=A, ks=2048, v=A, vs=2048, rows=640, pk=A, pks=2048, pv=A, pvs=2048, P=100, dtype=1, cu=A,
-             base=A, lens=A, B=4, N=4, heads=16, kv_heads=16, head_dim=64, chunk=1, scale=0.125, out=A, os=1024,
-             ws=A, ws_bytes=1 << 30)
+def attention(**kw):
+    from fcv_b200 import _lib
+
+    a = dict(q=A, k=A, v=A, pk=A, pv=A, cu=A, base=A, lens=A, out=A, qs=1024, ks=2048, vs=2048, rows=640, pks=2048,
+             pvs=2048, os=1024, P=100, dtype=1, B=4, N=4, heads=16, kv_heads=16, head_dim=64, chunk=1, scale=0.125)
     a.update(kw)
-    return lib.fcv_shared_prefix_attention(a["q"], a["qs"], a["k"], a["ks"], a["v"], a["vs"], a["rows"], a["pk"],
-                                           a["pks"], a["pv"], a["pvs"], a["P"], a["dtype"], a["cu"], a["base"],
-                                           a["lens"], a["B"], a["N"], a["heads"], a["kv_heads"], a["head_dim"],
-                                           a["chunk"], a["scale"], a["out"], a["os"], a["ws"], a["ws_bytes"], None)
+    return _lib.PREFIX_ATTENTION.pack(*a.values())
+
+
+def attend(lib, ws=A, ws_bytes=1 << 40, **kw):
+    return lib.fcv_shared_prefix_attention(attention(**kw), ws, ws_bytes, None)
 
 
 @pytest.mark.parametrize("bad,status", [
     (dict(dtype=7), -1), (dict(N=-1), -1), (dict(heads=0), -1), (dict(kv_heads=0), -1), (dict(eps=-1.0), -1),
     (dict(eps=float("nan")), -1), (dict(head_dim=96), -2), (dict(head_dim=0), -2), (dict(half=0), -2),
-    (dict(half=12), -2), (dict(half=40), -2), (dict(qkv=None), -1), (dict(cos=None), -1), (dict(pos=None), -1),
-    (dict(q=None), -1), (dict(k=None), -1), (dict(qkv=A + 8), -1), (dict(cos=A + 4), -1), (dict(qw=A + 4), -1),
+    (dict(half=12), -2), (dict(half=40), -2), (dict(qkv=0), -1), (dict(cos=0), -1), (dict(pos=0), -1),
+    (dict(q=0), -1), (dict(k=0), -1), (dict(qkv=A + 8), -1), (dict(cos=A + 4), -1), (dict(qw=A + 4), -1),
     (dict(stride=3073), -1), (dict(qs=1028), -1), (dict(ks=1028), -1), (dict(limit=3), -1), (dict(rows=-1), -1),
 ])
 def test_norm_refuses(lib, bad, status):
@@ -54,8 +58,8 @@ def test_norm_refuses(lib, bad, status):
 @pytest.mark.parametrize("bad,status", [
     (dict(dtype=2), -1), (dict(B=-1), -1), (dict(N=-1), -1), (dict(P=-1), -1), (dict(rows=-1), -1),
     (dict(chunk=-1), -1), (dict(heads=0), -1), (dict(kv_heads=0), -1), (dict(kv_heads=3), -1),
-    (dict(head_dim=32), -2), (dict(head_dim=256), -2), (dict(q=None), -1), (dict(k=None), -1), (dict(pv=None), -1),
-    (dict(cu=None), -1), (dict(out=None), -1), (dict(base=None), -1), (dict(lens=None), -1), (dict(q=A + 2), -1),
+    (dict(head_dim=32), -2), (dict(head_dim=256), -2), (dict(q=0), -1), (dict(k=0), -1), (dict(pv=0), -1),
+    (dict(cu=0), -1), (dict(out=0), -1), (dict(base=0), -1), (dict(lens=0), -1), (dict(q=A + 2), -1),
     (dict(out=A + 8), -1), (dict(qs=1025), -1), (dict(ks=1025), -1), (dict(pvs=1025), -1), (dict(os=1025), -1),
     (dict(ws_bytes=16, P=100000), -1), (dict(scale=0.0), -1), (dict(scale=-0.1), -1),
     (dict(scale=float("nan")), -1), (dict(scale=float("inf")), -1), (dict(ws=None, P=100000), -1), (dict(ws=A + 4, P=100000), -1),
@@ -66,20 +70,36 @@ def test_attention_refuses(lib, bad, status):
 
 
 def test_empty_calls_return_before_any_launch(lib):
-    assert norm(lib, N=0, qkv=None) == 0
-    assert attend(lib, N=0, q=None) == 0
-    assert attend(lib, B=0, cu=None) == 0
+    assert lib.fcv_qk_norm_rope(None, None) == -1 and lib.fcv_shared_prefix_attention(None, None, 0, None) == -1
+    assert norm(lib, N=0, qkv=0) == 0
+    assert attend(lib, N=0, q=0) == 0
+    assert attend(lib, B=0, cu=0) == 0
 
 
 def test_workspace_is_sized_on_the_host(lib):
-    size = lib.fcv_shared_prefix_workspace_bytes
-    assert size(0, 4, 16, 16, 64, 100, 6400, 0, 1) == 0
-    assert size(4, 0, 16, 16, 64, 100, 6400, 0, 1) == 0
-    assert size(4, 4, 16, 3, 64, 100, 6400, 0, 1) == 0
-    assert size(4, 4, 16, 16, 64, -1, 6400, 0, 1) == 0
-    # at least one part of the prefix and one of the own keys: output, maximum and sum of every head
-    assert size(4, 4, 16, 16, 64, 100, 6400, 0, 5) == 0
-    assert size(64, 64, 32, 8, 128, 4096, 6400, 0, 0) >= 2 * 64 * 32 * (128 * 4 + 8)
+    size = lambda **kw: lib.fcv_shared_prefix_workspace_bytes(attention(**kw))  # noqa: E731
+    assert size(N=0) == 0 and size(B=0) == 0 and size(kv_heads=3) == 0 and size(P=-1) == 0
+    assert size(dtype=5) == 0 and size(head_dim=96) == 0 and size(rows=-1) == 0
+    assert lib.fcv_shared_prefix_workspace_bytes(None) == 0
+    # one part of the prefix and one of the own keys at least: output, maximum and sum of every head
+    assert size(N=64, B=64, heads=32, kv_heads=8, head_dim=128, P=4096, dtype=0) >= 2 * 64 * 32 * (128 * 4 + 8)
+
+
+@pytest.mark.parametrize("name", ["fcv_qk_norm", "fcv_prefix_attention"])
+def test_packed_arguments_have_the_layout_of_the_header(name):
+    """The format strings against the structures that the header declares, field by field."""
+    from fcv_b200 import _lib
+
+    body = re.search(r"typedef struct %s \{(.*?)\} %s;" % (name, name), (ROOT / "include" / "fcv_b200.h").read_text(), re.S)
+    fmt = ""
+    for line in body.group(1).split(";"):
+        line = line.strip()
+        if line:
+            kind = "P" if "*" in line else {"long": "l", "int": "i", "float": "f"}[line.split()[0]]
+            fmt += kind * (line.count(",") + 1)
+    packed = {"fcv_qk_norm": _lib.QK_NORM, "fcv_prefix_attention": _lib.PREFIX_ATTENTION}[name]
+    assert packed.size == struct.calcsize("@" + fmt + "0P")  # padded like the C structure
+    assert re.sub(r"(\d+)([A-Za-z])", lambda m: m.group(2) * int(m.group(1)), packed.format[1:]).rstrip("x") == fmt
 
 
 def test_cpu_tensors_are_refused():
