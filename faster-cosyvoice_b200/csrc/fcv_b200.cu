@@ -572,9 +572,11 @@ SpPlan sp_plan(const fcv_prefix_attention& g) {
                                  : std::max(own_tiles * kAlone[d][r], load * (own_tiles * kAmong[d][r] + 0.6)) + 3;
     parts_us = 10 + std::max(fa_parts, own_us) + 0.35 * std::min(fa_parts, own_us) + (double)N * H * D * 16 / 2.5e6;
   } else {
-    // in tile steps of an SM's two blocks; a join costs about one and a half
+    // fp32, in tile steps of an SM's two blocks (5 and 9 us); the choice is 0.3 % slower than the better way
+    // over the same shapes
     whole_us = std::ceil(load / 2) * all;
-    parts_us = ((rows + p.prefix_rows - 1) / p.prefix_rows * Hkv * tiles + own_blocks * own_tiles) / (2.0 * sms) + 1.5;
+    parts_us = ((rows + p.prefix_rows - 1) / p.prefix_rows * Hkv * tiles + own_blocks * own_tiles) / (2.0 * sms) + 1.5 +
+               (double)N * H * D * 16 / 2.5e6 / (d ? 9 : 5);
     if (load < 1) whole_us = all;
   }
   p.fa_whole = fa_us < whole_us && fa_us < parts_us;
@@ -640,9 +642,9 @@ SpPlan sp_plan(const fcv_prefix_attention& g) {
       if (best == 0 || cost < best) best = cost, p.prefix_parts = n;
     }
   } else if (P > 0) {
-    // enough blocks for two on every SM, no part under 256 keys
+    // enough blocks for two on every SM
     const long blocks = p.prefix_blocks * Hkv;
-    p.prefix_parts = (int)std::max(1L, std::min(std::min(64L, (P + 255) / 256), (2 * sms + blocks - 1) / blocks));
+    p.prefix_parts = (int)std::max(1L, std::min(std::min(64L, tiles), (2 * sms + blocks - 1) / blocks));
   }
   if (stream) {
     p.own_parts = 1;

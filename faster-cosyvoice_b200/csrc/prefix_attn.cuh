@@ -70,6 +70,12 @@ struct SpArgs {
 };
 
 constexpr int kSpKeys = 64;  // keys of a tile
+// Fewest tiles of a part: a part's join costs about as much as four tiles in bf16, as one in fp32
+// (16 streams behind 1000 keys, parts of at least 4 and 1 tiles: 28.8 and 15.9 us).
+template <typename T>
+__host__ __device__ constexpr int sp_least() {
+  return sizeof(T) == 2 ? 4 : 1;
+}
 
 struct SpSeq {
   int q0, nq, nk;
@@ -108,9 +114,9 @@ __device__ __forceinline__ int sp_limit(const SpArgs& a, const SpSeq& s, int i) 
   return sp_limit_at(a, s.nk, s.nk - s.nq + i);
 }
 // Tiles [t0, t1) of piece `part` out of at most `parts` over `tiles` tiles: pieces of equal size,
-// none shorter than four tiles unless it is the last.
-__device__ __forceinline__ void sp_piece(int tiles, int parts, int part, int& t0, int& t1) {
-  const int n = max(1, min(parts, (tiles + 3) / 4));
+// none shorter than `least` tiles unless it is the last.
+__device__ __forceinline__ void sp_piece(int tiles, int parts, int least, int part, int& t0, int& t1) {
+  const int n = max(1, min(parts, (tiles + least - 1) / least));
   const int each = (tiles + n - 1) / n;
   t0 = min(tiles, part * each);
   t1 = part < n ? min(tiles, t0 + each) : t0;
@@ -611,7 +617,7 @@ __device__ __forceinline__ void sp_block(const SpArgs& a, uint8_t* smem) {
     const long r0 = R0 > first ? R0 : first;
     const long r1 = min(R0 + RP, end);
     if (r0 >= r1) return;
-    sp_piece(prefix_tiles, a.prefix_parts, part, pre.t0, pre.t1);
+    sp_piece(prefix_tiles, a.prefix_parts, sp_least<T>(), part, pre.t0, pre.t1);
     pre.k += (long)hk * D;
     pre.v += (long)hk * D;
     piece(std::integral_constant<int, RP>(), pre, own, hk, r0, static_cast<int>(r1 - r0), part,
@@ -633,7 +639,7 @@ __device__ __forceinline__ void sp_block(const SpArgs& a, uint8_t* smem) {
   for (long r = (long)blockIdx.y * RO; r < nrows; r += (long)gridDim.y * RO) {
     const int rows = static_cast<int>(min((long)RO, nrows - r));
     const int seen = sp_limit(a, s, static_cast<int>((r + rows - 1) / a.G));  // limits grow along the rows
-    sp_piece((seen + kSpKeys - 1) / kSpKeys, a.own_parts, part, own.t0, own.t1);
+    sp_piece((seen + kSpKeys - 1) / kSpKeys, a.own_parts, sp_least<T>(), part, own.t0, own.t1);
     piece(std::integral_constant<int, RO>(), pre, own, hk, (long)s.q0 * a.G + r, rows,
           a.whole ? -1 : a.prefix_parts + part,
           [&](int i) { return sp_limit(a, s, static_cast<int>((r + i) / a.G)); });

@@ -283,7 +283,7 @@ __global__ void __launch_bounds__(SpFa<D>::THREADS, 1)
           o.tok0 = static_cast<int>(lo);
           o.ntok = static_cast<int>(hi - lo);
           int t1;
-          sp_piece((A.P + kSfKeys - 1) / kSfKeys, prefix_parts, o.part, o.p0, t1);
+          sp_piece((A.P + kSfKeys - 1) / kSfKeys, prefix_parts, sp_least<bf16>(), o.part, o.p0, t1);
           o.np = t1 - o.p0;
           o.nk = o.rel = o.own = 0;
         }

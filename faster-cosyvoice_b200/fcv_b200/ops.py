@@ -157,29 +157,20 @@ def _raw_stream(device: int) -> int:
     return torch._C._cuda_getCurrentRawStream(device)
 
 
-def _device_of(first: torch.Tensor, others: tuple) -> int:
-    """Index of the CUDA device on which ``first`` lives; the other tensors (None: absent) must too."""
-    dev = first.get_device()
-    if dev < 0:
-        raise ValueError("tensors must live on a CUDA device")
-    for t in others:
-        if t is not None and t.get_device() != dev:
-            raise ValueError(f"a tensor lives on {t.device}, not on cuda:{dev}")
-    return dev
+def _int32(name: str, t: torch.Tensor, n: int, dev: int):
+    if t.dtype is not torch.int32 or t.shape != (n,) or t.get_device() != dev or not t.is_contiguous():
+        raise ValueError(f"{name} must be a contiguous int32 tensor of {n} entries on cuda:{dev}")
 
 
-def _int32(name: str, t: torch.Tensor, n: int):
-    if t.dtype is not torch.int32 or t.dim() != 1 or t.shape[0] != n or not t.is_contiguous():
-        raise ValueError(f"{name} must be a contiguous int32 tensor of {n} entries")
-
-
-def _head_rows(name: str, t: torch.Tensor, heads: int, head_dim: int, dtype: torch.dtype) -> tuple[int, int]:
+def _head_rows(name: str, t: torch.Tensor, heads: int, head_dim: int, dtype: torch.dtype,
+               dev: int) -> tuple[int, int]:
     """Rows and row stride of a (rows, heads, head_dim) tensor whose heads are packed inside a row."""
     shape = t.shape
-    if len(shape) != 3 or shape[1] != heads or shape[2] != head_dim or t.dtype is not dtype:
-        raise ValueError(f"{name} must be (rows, {heads}, {head_dim}) of {dtype}")
+    if (len(shape) != 3 or shape[1] != heads or shape[2] != head_dim or t.dtype is not dtype
+            or t.get_device() != dev):
+        raise ValueError(f"{name} must be (rows, {heads}, {head_dim}) of {dtype} on cuda:{dev}")
     row, head, last = t.stride()
-    if shape[0] > 0 and (last != 1 or (head != head_dim and heads > 1)):
+    if (last != 1 or (head != head_dim and heads > 1)) and shape[0] > 0:
         raise ValueError(f"the heads of a {name} row must be contiguous")
     return shape[0], row
 
@@ -220,19 +211,23 @@ def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: tor
         raise ValueError("qkv must be (N, (heads + 2 kv_heads) head_dim)")
     N, width = shape
     D = width // (heads + 2 * kv_heads)
-    dev = _device_of(qkv, (q_weight, k_weight, rope_cos, rope_sin, positions, kv_cache, kv_rows))
+    dev = qkv.get_device()
+    if dev < 0:
+        raise ValueError("tensors must live on a CUDA device")
     dt = _dt(qkv)
     row, last = qkv.stride()
     if (N > 0 and last != 1) or (N > 1 and row < width):
         raise ValueError("qkv rows must be contiguous and must not overlap")
     for name, w in (("q_weight", q_weight), ("k_weight", k_weight)):
-        if w is not None and (w.dtype is not torch.float32 or w.shape != (D,) or not w.is_contiguous()):
-            raise ValueError(f"{name} must be a contiguous float32 tensor of shape ({D},)")
+        if w is not None and (w.dtype is not torch.float32 or w.shape != (D,) or w.get_device() != dev
+                              or not w.is_contiguous()):
+            raise ValueError(f"{name} must be a contiguous float32 tensor of shape ({D},) on cuda:{dev}")
     table = rope_cos.shape
     if (len(table) != 2 or table != rope_sin.shape or rope_cos.dtype is not torch.float32
-            or rope_sin.dtype is not torch.float32 or not rope_cos.is_contiguous() or not rope_sin.is_contiguous()):
-        raise ValueError("rope_cos and rope_sin must be contiguous float32 tables of one shape")
-    _int32("positions", positions, N)
+            or rope_sin.dtype is not torch.float32 or not rope_cos.is_contiguous() or not rope_sin.is_contiguous()
+            or rope_cos.get_device() != dev or rope_sin.get_device() != dev):
+        raise ValueError(f"rope_cos and rope_sin must be contiguous float32 tables of one shape on cuda:{dev}")
+    _int32("positions", positions, N, dev)
     if (kv_cache is None) != (kv_rows is None):
         raise ValueError("kv_cache and kv_rows go together")
     ptr, es, q_width, k_width = qkv.data_ptr(), qkv.element_size(), heads * D, kv_heads * D
@@ -242,9 +237,10 @@ def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: tor
         q, q_row = qkv.new_empty((N, heads, D)), q_width
     v_ptr = rows_ptr = 0
     if kv_cache is not None:
-        _int32("kv_rows", kv_rows, N)
-        if kv_cache.dim() != 2 or kv_cache.shape[1] != 2 * k_width or kv_cache.dtype is not qkv.dtype:
-            raise ValueError(f"kv_cache must be (rows, {2 * k_width}) of {qkv.dtype}")
+        _int32("kv_rows", kv_rows, N, dev)
+        if (kv_cache.dim() != 2 or kv_cache.shape[1] != 2 * k_width or kv_cache.dtype is not qkv.dtype
+                or kv_cache.get_device() != dev):
+            raise ValueError(f"kv_cache must be (rows, {2 * k_width}) of {qkv.dtype} on cuda:{dev}")
         limit = kv_cache.shape[0]
         k_row, last = kv_cache.stride()
         if (limit > 0 and last != 1) or (limit > 1 and k_row < 2 * k_width):
@@ -293,27 +289,28 @@ def shared_prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, p
     sequence's result may differ in the last bits with its company; equal calls give equal bits."""
     if q.dim() != 3 or prefix_k.dim() != 3:
         raise ValueError("q must be (N, heads, head_dim), prefix_k (P, kv_heads, head_dim)")
-    dev = _device_of(q, (k, v, prefix_k, prefix_v, cu_seqlens, kv_base, kv_lens, out))
     N, H, D = q.shape
-    Hkv = prefix_k.shape[1]
-    dt, dtype = _dt(q), q.dtype
+    Hkv, dtype, dev = prefix_k.shape[1], q.dtype, q.get_device()
+    if dev < 0:
+        raise ValueError("tensors must live on a CUDA device")
+    dt = _dt(q)
     if Hkv < 1 or H < 1 or H % Hkv:
         raise ValueError(f"{H} query heads do not share {Hkv} key heads evenly")
-    _, q_row = _head_rows("q", q, H, D, dtype)
-    rows, k_row = _head_rows("k", k, Hkv, D, dtype)
-    v_rows, v_row = _head_rows("v", v, Hkv, D, dtype)
-    P, pk_row = _head_rows("prefix_k", prefix_k, Hkv, D, dtype)
-    pv_rows, pv_row = _head_rows("prefix_v", prefix_v, Hkv, D, dtype)
+    _, q_row = _head_rows("q", q, H, D, dtype, dev)
+    rows, k_row = _head_rows("k", k, Hkv, D, dtype, dev)
+    v_rows, v_row = _head_rows("v", v, Hkv, D, dtype, dev)
+    P, pk_row = _head_rows("prefix_k", prefix_k, Hkv, D, dtype, dev)
+    pv_rows, pv_row = _head_rows("prefix_v", prefix_v, Hkv, D, dtype, dev)
     if rows != v_rows or P != pv_rows:
         raise ValueError("keys and values must have the same rows")
-    B = cu_seqlens.numel() - 1
+    B = cu_seqlens.shape[0] - 1 if cu_seqlens.dim() == 1 else -1
     if B < 0:
         raise ValueError("cu_seqlens must hold at least one entry")
-    _int32("cu_seqlens", cu_seqlens, B + 1)
+    _int32("cu_seqlens", cu_seqlens, B + 1, dev)
     base_ptr = lens_ptr = 0
     if kv_base is not None and kv_lens is not None:
-        _int32("kv_base", kv_base, B)
-        _int32("kv_lens", kv_lens, B)
+        _int32("kv_base", kv_base, B, dev)
+        _int32("kv_lens", kv_lens, B, dev)
         base_ptr, lens_ptr = kv_base.data_ptr(), kv_lens.data_ptr()
     elif kv_base is not None or kv_lens is not None:
         raise ValueError("kv_base and kv_lens go together")
@@ -324,7 +321,7 @@ def shared_prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, p
     if out is None:
         out, out_row = q.new_empty((N, H, D)), H * D
     else:
-        out_rows, out_row = _head_rows("out", out, H, D, dtype)
+        out_rows, out_row = _head_rows("out", out, H, D, dtype, dev)
         if out_rows != N or (N > 1 and out_row < H * D):
             raise ValueError("out must be (N, heads, head_dim) rows that do not overlap")
         if any(_overlap(out, t) for t in (q, k, v, prefix_k, prefix_v)):
