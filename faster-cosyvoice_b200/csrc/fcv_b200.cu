@@ -541,9 +541,13 @@ SpPlan sp_plan(const fcv_prefix_attention& g) {
   const long tile = G <= 128 ? 128 / G : 1, block = (D == 64 ? 3 : 2) * tile;  // tokens
   const long sms = num_sms();
   const long tiles = (P + kSpKeys - 1) / kSpKeys;
-  const long own_len = packed ? (q_len + 1) / 2 : std::min(kv_rows / B, 4096L) / 2;
+  const long own_len = packed ? (g.chunk == 0 ? q_len : (q_len + 1) / 2) : std::min(kv_rows / B, 4096L) / 2;
   const long own_tiles = std::max(1L, (own_len + kSpKeys - 1) / kSpKeys);
-  const bool tensor = bf && G <= 128;
+  // the tensor-core kernels load by TMA, whose rows may not overlap (expanded tensors)
+  auto apart = [](long n, long stride, long width) { return n <= 1 || stride >= width; };
+  const bool tensor = bf && G <= 128 && apart(N, g.q_stride, (long)H * D) && apart(P, g.prefix_k_stride, (long)Hkv * D) &&
+                      apart(P, g.prefix_v_stride, (long)Hkv * D) && apart(kv_rows, g.k_stride, (long)Hkv * D) &&
+                      apart(kv_rows, g.v_stride, (long)Hkv * D);
   p.prefix_rows = rows <= 16 ? 16 : 64;
   p.own_rows = own <= 16 ? 16 : 64;
   const bool stream = tensor && G <= 16 && own <= 16;
@@ -574,7 +578,7 @@ SpPlan sp_plan(const fcv_prefix_attention& g) {
   } else {
     // fp32, in tile steps of an SM's two blocks (5 and 9 us); the choice is 0.3 % slower than the better way
     // over the same shapes
-    whole_us = std::ceil(load / 2) * all;
+    whole_us = (load / 2 + 0.4) * all;
     parts_us = ((rows + p.prefix_rows - 1) / p.prefix_rows * Hkv * tiles + own_blocks * own_tiles) / (2.0 * sms) + 1.5 +
                (double)N * H * D * 16 / 2.5e6 / (d ? 9 : 5);
     if (load < 1) whole_us = all;

@@ -407,6 +407,70 @@ def test_attention_refuses_bad_tensors():
     assert none.shape == (0, 4, 64)
 
 
+# (query lengths, keys before them, prefix, H, Hkv, D) and the kernels that a bf16 call launches
+WAYS = {
+    "whole, few rows": (([1] * 4, [0, 5, 30, 36], 200, 16, 16, 64), 1),
+    "whole, 50-row chunks": (([50] * 12, [0] * 12, 150, 16, 16, 64), 1),
+    "whole, tensor cores, heads of 64": (([300, 411, 1, 260] * 4, None, 777, 14, 2, 64), 2),
+    "whole, tensor cores, heads of 128": (([300, 411, 1, 260] * 4, None, 500, 32, 8, 128), 2),
+    "parts, own keys streamed, heads of 64": (([1] * 40, list(range(0, 400, 10)), 6000, 16, 4, 64), 3),
+    "parts, own keys streamed, heads of 128": (([1] * 40, list(range(0, 400, 10)), 6000, 32, 8, 128), 3),
+    "parts, shared SMs picked on the device": (([1] * 130, [i % 97 for i in range(130)], 16000, 32, 8, 128), 3),
+    "parts, several queries streamed": (([2, 3, 1, 0, 4] * 6, [70] * 30, 5000, 16, 4, 64), 3),
+    "parts, rows of a sequence in blocks": (([50, 3, 77], [100, 0, 9], 9000, 16, 16, 64), 3),
+    "parts, 20 heads to a key head": (([1, 2, 1], [100, 0, 900], 9000, 20, 1, 128), 3),
+    "130 heads to a key head": (([1, 5], [40, 0], 700, 130, 1, 64), 2),
+}
+
+
+@pytest.mark.parametrize("way", list(WAYS))
+@pytest.mark.parametrize("chunk", [1, 0])
+def test_every_way_of_cutting(way, chunk):
+    from fcv_b200 import _lib
+
+    (q_lens, past, P, H, Hkv, D), launches = WAYS[way]
+    count = _lib.lib().fcv_launch_count
+    before = count()
+    run_case(q_lens, past, P, H, Hkv, D, torch.bfloat16, chunk, 7)
+    assert (count() - before) / 2 == launches  # run_case calls twice
+    run_case(q_lens[:8], past and past[:8], min(P, 900), H, Hkv, D, torch.float32, chunk, 8)
+
+
+def test_expanded_rows():
+    """Rows of stride 0 (a TMA tensor may not have them): one key repeated is one key."""
+    H, Hkv, D = 8, 2, 64
+    g = gen(51)
+    q = torch.randn(300, H, D, generator=g, device=DEV).bfloat16()
+    one = torch.randn(1, Hkv, D, generator=g, device=DEV).bfloat16()
+    cu = torch.tensor([0, 300], dtype=torch.int32, device=DEV)
+    none = torch.zeros(1, dtype=torch.int32, device=DEV)
+    got = ops().shared_prefix_attention(q, one[:0], one[:0], one.expand(2000, -1, -1), one.expand(2000, -1, -1), cu,
+                                        none, none)
+    want = one.repeat_interleave(H // Hkv, 1).expand(300, -1, -1).double()
+    assert ((got.double() - want).abs() <= 2 * 2.0 ** -8 * want.abs()).all()
+
+
+@pytest.mark.parametrize("value", [float("nan"), float("inf")])
+@pytest.mark.parametrize("q_lens,past,P,D", [([1, 1, 1], [40, 70, 3], 100, 64), ([1, 1, 1], [40, 70, 3], 6000, 128),
+                                             ([200, 150, 90], None, 300, 64), ([300, 250, 90], None, 300, 128),
+                                             ([40, 33, 20], [0, 70, 3], 6000, 64)])
+def test_not_a_number_in_a_key_stays_with_the_rows_that_see_it(value, q_lens, past, P, D):
+    for dtype in (torch.bfloat16, torch.float32):
+        args, base, lens = attention_inputs(q_lens, past, P, 8, 2, D, dtype, 61, poison=past is not None)
+        clean = ops().shared_prefix_attention(**args)
+        at = lens[1] - 2  # the last key but one of the second sequence: seen by its last two queries
+        args["k"][base[1] + at, 0, 5] = value
+        got = ops().shared_prefix_attention(**args)
+        rows = torch.arange(sum(q_lens[:1]) + max(0, q_lens[1] - 2), sum(q_lens[:2]), device=DEV)
+        if value != value:
+            assert torch.isnan(got[rows][:, :4]).all()  # the four query heads of key head 0
+        else:  # a score of +inf or -inf by the query's sign: NaN, or the key left out
+            plus = args["q"][rows][:, :4, 5] > 0
+            assert torch.isnan(got[rows][:, :4][plus]).all() and torch.isfinite(got[rows][:, :4][~plus]).all()
+        got[rows, :4] = clean[rows, :4]
+        assert torch.equal(got, clean)
+
+
 def test_agrees_with_ragged_attention_on_whole_documents():
     """A batch whose documents start with the same rows: the rows behind them, computed with the shared
     keys, agree with the packed attention of the whole documents."""
@@ -518,6 +582,26 @@ def test_side_stream_and_graph_replay_with_new_lengths():
     ref = attention_ref(args["q"], args["k"], args["v"], args["prefix_k"], args["prefix_v"], [1] * 6, base,
                         [1, 1, 1, 50, 2, 201], 1, D ** -0.5)
     check_attention(outs[0][0], ref, 701)
+
+
+def test_replayed_decode_steps_follow_the_lengths():
+    """Prefix parts and streamed own keys side by side in a graph: each replay recomputes the cut."""
+    o = ops()
+    for P, B in ((9000, 24), (16000, 130)):
+        args, base, lens = attention_inputs([1] * B, [(37 * b) % 211 for b in range(B)], P, 32, 8, 128, torch.bfloat16, 71)
+        o.shared_prefix_attention(**args)
+        gr = torch.cuda.CUDAGraph()
+        with torch.cuda.graph(gr):
+            y = o.shared_prefix_attention(**args)
+        for new in (lens, [1] * B, [max(1, n - 7 * (b % 5)) for b, n in enumerate(lens)], [0] * B):
+            args["kv_lens"].copy_(torch.tensor(new, dtype=torch.int32))
+            for _ in range(3):
+                gr.replay()
+            eager = o.shared_prefix_attention(**args)
+            assert torch.equal(y, eager)
+            ref = attention_ref(args["q"], args["k"], args["v"], args["prefix_k"], args["prefix_v"], [1] * B, base, new, 1,
+                                128 ** -0.5)
+            check_attention(y, ref, P + max(new))
 
 
 def test_two_calls_at_once_on_two_streams():
