@@ -1396,8 +1396,8 @@ int fcv_shared_prefix_attention(const fcv_prefix_attention* g, void* workspace, 
       a.split.own_us[i] = left > 0 ? std::max(p.split.floor_us, p.split.unit_us / left) : 0.f;
     }
     // A short prefix is given the few SMs on which it takes no longer than the own keys could (by the
-    // rows of k, at most 30 us): the device's choice costs 6 us (64 streams behind 4096 keys: 50 us
-    // against 44), and being wrong costs little.
+    // rows of k, at most 30 us): the device's choice costs 3 us (64 streams behind 4096 keys: 46.5 us
+    // against 43.6), and being wrong costs little.
     const float units = (float)kv_rows * kv_heads / kSpKeys + (float)B * kv_heads * (kSsItem + 1);
     const float most = std::min(30.f, std::max(12.f, 8.f + units * a.split.floor_us));
     for (int i = 0; i < a.split.n; ++i) {

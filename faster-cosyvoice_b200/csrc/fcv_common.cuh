@@ -16,7 +16,8 @@ namespace fcv {
 
 typedef __nv_bfloat16 bf16;
 
-// Device error word: first error code wins.  Codes: 1xx GEMM, 2xx attention.
+// Device error word: first error code wins.  Codes: 1xx GEMM, 2xx attention, 601-602 rows of the
+// query/key norm, 611-612 sequences of the shared-prefix attention, 638-665 its bounded waits.
 __device__ int g_device_error = 0;
 
 __device__ __forceinline__ void record_error(int code) { atomicCAS(&g_device_error, 0, code); }

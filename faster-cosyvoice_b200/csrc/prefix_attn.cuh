@@ -12,6 +12,12 @@
 // key is read once for 64 rows, not once for every sequence -- and the own keys run per sequence.
 // Each piece of keys leaves a running maximum, sum and unnormalised output in float32; a second
 // kernel joins the pieces of a row.
+//
+// This file has the kernel for few rows in bf16 (mma.sync: 16 to 64 rows to a block, bound by the
+// latency of a key tile, 0.43 us for 16 rows of 64 values, 0.74 us of 128) and for all of float32 (CUDA
+// cores, bound by the FMA pipe: 354 us for 8 documents of 243 to 600 rows behind 250 keys, 16 heads of
+// 64, 30 TFLOP/s), and the join.  prefix_fa.cuh has the tensor-core kernel for many rows,
+// prefix_stream.cuh the one for the own keys of decode steps.
 #pragma once
 
 #include <type_traits>
@@ -655,7 +661,8 @@ __global__ void __launch_bounds__(128) sp_pieces_kernel(const SpArgs a) {
 }
 
 // Own parts left by sp_stream_kernel.  The (sequence, row block, key head) items lie end to end, each
-// kSsItem units for its own cost and one for every key tile, and are cut into equal stretches.
+// kSsItem units for its own cost (start, join) and one for every key tile, and are cut into equal
+// stretches (64 sequences of 1 to 1023 keys: 79 us when only tiles count, 62 with three units an item).
 constexpr int kSsItem = 3;
 struct SsCount {
   int blocks, tiles;  // row blocks of 16 / G tokens; key tiles of each item
@@ -684,7 +691,9 @@ __device__ __forceinline__ int sp_pick(const SpSplit& s, long units) {
   float best_us = 0.f;
   const float u = static_cast<float>(units);
   for (int i = 0; i < s.n; ++i) {
-    const float us = s.own_us[i] > 0.f ? fmaxf(s.fa_us[i], u * s.own_us[i]) : s.fa_us[i] + u * s.floor_us;
+    // rounded one by one: every kernel has to come to the same figure
+    const float us = s.own_us[i] > 0.f ? fmaxf(s.fa_us[i], __fmul_rn(u, s.own_us[i]))
+                                       : __fadd_rn(s.fa_us[i], __fmul_rn(u, s.floor_us));
     if (i == 0 || us < best_us) best = i, best_us = us;
   }
   return best;
@@ -694,28 +703,24 @@ __device__ __forceinline__ int sp_pick_cuts(const SpSplit& s, int i) {
 }
 
 // Joins the parts of a row: one warp per (token, head).  Its loads are a chain of round trips (the
-// token's sequence, the parts' maxima and sums, their outputs), so what can be read at once is.
+// token's sequence, the parts' maxima and sums, their outputs), so what can be read at once is: part by
+// part it took 24 us for 2048 rows of 17 parts, like this 7 us for the 5 parts that they have now.
 template <typename T, int D>
 __global__ void __launch_bounds__(256) sp_join_kernel(const SpArgs a) {
-  griddep_wait();
-  griddep_launch();
   const int lane = threadIdx.x & 31;
   const long w = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
-  const int token = static_cast<int>(w / a.H);
-  if (token >= a.N) return;
+  const int token = static_cast<int>(min(w / a.H, (long)a.N));
   const int head = static_cast<int>(w - (long)token * a.H);
   const long step = (long)a.N * a.H;
-  // own parts: all of them, or (cuts) one in the row's own place or one in each stretch that the item meets
-  int own = a.own_parts, first = -1, prefix_parts = a.prefix_parts;
-  long slot_row = 0;
+  // The caller's arrays may be read before the wait: the kernels that leave the parts launch this one
+  // after their own wait (or the one beside them did) for whatever was on the stream before the call.
   const int begin = a.cu[0], end = a.cu[a.B];
-  if (a.cuts > 0) {
-    own = 0;
+  int b = 0;
+  SpSeq s{};
+  if (a.cuts > 0 && token < a.N) {
     // the token's sequence: its own number when every sequence has one query
-    int b = min(token, a.B - 1);
-    SpSeq s = sp_sequence(a, b, false);
-    long start = a.tile_start[b];
-    const long total = a.tile_start[a.B];
+    b = min(token, a.B - 1);
+    s = sp_sequence(a, b, false);
     if (s.q0 > token || s.q0 + s.nq <= token) {
       int lo = 0, hi = a.B - 1;
       while (lo < hi) {
@@ -723,9 +728,20 @@ __global__ void __launch_bounds__(256) sp_join_kernel(const SpArgs a) {
         if (a.cu[mid + 1] > token) hi = mid;
         else lo = mid + 1;
       }
-      s = sp_sequence(a, lo, false);
-      start = a.tile_start[lo];
+      b = lo;
+      s = sp_sequence(a, b, false);
     }
+  }
+  griddep_wait();
+  griddep_launch();
+  if (token >= a.N || token < begin || token >= end) return;  // rows behind the last sequence stay
+  // own parts: all of them, or (cuts) one in the row's own place or one in each stretch that the item meets
+  int own = a.own_parts, first = -1, prefix_parts = a.prefix_parts;
+  long slot_row = 0;
+  if (a.cuts > 0) {
+    own = 0;
+    const long total = a.tile_start[a.B];
+    long start = a.tile_start[b];
     const SsCount c = ss_count(a, s.nq, s.nk);
     const int i = token - s.q0;
     int cuts = a.cuts;
@@ -744,7 +760,6 @@ __global__ void __launch_bounds__(256) sp_join_kernel(const SpArgs a) {
       slot_row = (i - rb * per) * a.G + (head - hk * a.G);
     }
   }
-  if (token < begin || token >= end) return;  // rows behind the last sequence stay
   const int parts = prefix_parts + own;
   // part p of the row: its index among the stored maxima and sums (and, times D, among the outputs)
   auto place = [&](int p, const float2*& ml, const float*& o) {

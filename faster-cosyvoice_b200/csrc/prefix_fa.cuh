@@ -14,9 +14,17 @@
 // S_t = Q_t K^T (128 x 64) and O_t (128 x D) live in tensor memory, P_t goes back there as bf16;
 // S of the next key tile is issued before P V of the present one.
 //
-// Bound: per query tile and 64 keys, 8192 exponentials (16 per clock and SM: 512 clocks; a quarter
-// of them run as a polynomial on the FMA pipe) against 2 * 128 * 64 * D * 2 tensor FLOPs (48 clocks
-// per 128 x 64 x 16 MMA): at D = 64 the exponentials bound it, at D = 128 the two are alike.
+// Per query tile and 64 keys there are 8192 exponentials (16 per clock and SM: 512 clocks; a quarter
+// of them run as a polynomial on the FMA pipe) and 4 * 128 * 64 * D tensor FLOPs (48 clocks per 128 x
+// 64 x 16 MMA of S, at D = 128 64 clocks per 128 x 128 x 16 MMA of P V).  Neither bounds it: at D = 128
+// with two query tiles a step takes 2290 clocks, of which the MMAs fill 1280, and dropping the
+// exponentials, the MMAs, or both in a test build leaves 98, 89 and 62 % of the time -- the hand-overs
+// between softmax, issuer and tensor core (commit, mbarrier, wake-up) do.  Tensor memory allows no more
+// steps in flight: O takes 128 columns for each query tile.  Measured: 16 sequences of 700 to 1024
+// tokens behind 4096 keys, 32/8 heads of 128, 980 GFLOP: 990 us at burst clocks, 1110 us in a long run
+// (0.59 and 0.52 of the measured bf16 rates' burst figure, 0.64 of the sustained one).  Two threads to
+// a row (32 keys each, twice the warps) 1075 us; two S buffers with P over S, so that S of the next
+// tile and the store of P wait for nothing, 1000 us; both 1098 us.
 #pragma once
 
 #include "attn.cuh"

@@ -314,6 +314,8 @@ def shared_prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, p
         base_ptr, lens_ptr = kv_base.data_ptr(), kv_lens.data_ptr()
     elif kv_base is not None or kv_lens is not None:
         raise ValueError("kv_base and kv_lens go together")
+    elif rows < N:
+        raise ValueError("without kv_base, k and v must have a row for every query")
     if chunk < 0:
         raise ValueError("chunk must not be negative")
     if scale is None:

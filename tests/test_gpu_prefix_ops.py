@@ -393,7 +393,7 @@ def test_attention_refuses_bad_tensors():
         dict(k=args["k"][:-1]), dict(k=args["k"].float()), dict(v=args["v"][:, :1]),
         dict(prefix_v=args["prefix_v"][:3]), dict(cu_seqlens=args["cu_seqlens"].long()),
         dict(cu_seqlens=args["cu_seqlens"].cpu()), dict(kv_base=None), dict(kv_lens=args["kv_lens"][:1]),
-        dict(chunk=-1), dict(out=out[:4]), dict(out=out.float()), dict(out=q), dict(cu_seqlens=args["cu_seqlens"][:0]),
+        dict(chunk=-1), dict(kv_base=None, kv_lens=None, k=args["k"][:4], v=args["v"][:4]), dict(out=out[:4]), dict(out=out.float()), dict(out=q), dict(cu_seqlens=args["cu_seqlens"][:0]),
         dict(out=out[:1].expand(5, -1, -1)),
     ]
     for i, change in enumerate(bad):
