@@ -319,8 +319,8 @@ __device__ __forceinline__ void sp_mma_piece(const SpArgs& a, uint8_t* smem, con
     l1 = l1 * e1 + y1;
 #pragma unroll
     for (int i = 0; i < D / 8; ++i) o[i][0] *= e0, o[i][1] *= e0, o[i][2] *= e1, o[i][3] *= e1;
-    // P is rounded to bf16 for the product (half a step, 2^-9 relative, averaged over the keys);
-    // its sum stays in float32
+    // P is rounded to bf16 for the product (at most half a step, 2^-8 relative, averaged over the
+    // keys); its sum stays in float32
 #pragma unroll
     for (int kk = 0; kk < KW / 16; ++kk) {
       const uint32_t pf[4] = {pack_bf16x2(s[2 * kk][0], s[2 * kk][1]), pack_bf16x2(s[2 * kk][2], s[2 * kk][3]),

@@ -146,6 +146,18 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) qk_norm_rope_kern
     }
   }
   // queries, then keys (a step may hold the last of the one and the first of the other)
+  float wt[8];
+  auto weights = [&](const float* p) {
+    if (p) {
+      Vec8<float> t;
+      t.load(p + d0), t.get(wt);
+    } else {
+#pragma unroll
+      for (int i = 0; i < 8; ++i) wt[i] = 1.f;
+    }
+  };
+  bool of_q = part * HPW + sub < a.heads;
+  weights(of_q ? a.q_weight : a.k_weight);
   for (int base = part * HPW; base < units; base += U * step) {
     if (base != part * HPW) load(base, units);
 #pragma unroll
@@ -154,15 +166,11 @@ __global__ void __launch_bounds__(256, sizeof(T) == 2 ? 3 : 2) qk_norm_rope_kern
       if (h0 >= units) break;  // warp-uniform
       const int h = h0 + sub;
       const bool is_q = h < a.heads;
-      const float* wp = is_q ? a.q_weight : a.k_weight;
-      float x[8], wt[8];
-      if (wp) {
-        Vec8<float> t;
-        t.load(wp + d0), t.get(wt);
-      } else {
-#pragma unroll
-        for (int i = 0; i < 8; ++i) wt[i] = 1.f;
+      if (is_q != of_q) {  // the lane's last query head is behind it
+        weights(a.k_weight);
+        of_q = false;
       }
+      float x[8];
       v[u].get(x);
       float ss = 0.f;
 #pragma unroll

@@ -321,7 +321,7 @@ def shared_prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, p
     if scale is None:
         scale = D ** -0.5
     if out is None:
-        out, out_row = q.new_empty((N, H, D)), H * D
+        out, out_row = torch.empty_like(q) if q.is_contiguous() else q.new_empty((N, H, D)), H * D
     else:
         out_rows, out_row = _head_rows("out", out, H, D, dtype, dev)
         if out_rows != N or (N > 1 and out_row < H * D):

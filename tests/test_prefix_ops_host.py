@@ -24,8 +24,8 @@ def lib():
 def norm(lib, **kw):
     from fcv_b200 import _lib
 
-    a = dict(qkv=A, qw=A, kw=A, cos=A, sin=A, pos=A, q=A, k=A, v=0, kv_rows=0, stride=3072, qs=1024, ks=1024, vs=1024,
-             limit=4, dtype=1, N=4, heads=16, kv_heads=16, head_dim=64, rows=128, half=32, inter=1, eps=1e-6)
+    a = dict(qkv=A, qw=A, kw=A, cos=A, sin=A, pos=A, q=A, k=A, v=0, kv_rows=0, stride=1536, qs=512, ks=512, vs=512,
+             limit=4, dtype=1, N=4, heads=8, kv_heads=8, head_dim=64, rows=128, half=32, inter=1, eps=1e-6)
     a.update(kw)
     return lib.fcv_qk_norm_rope(_lib.QK_NORM.pack(*a.values()), None)
 
@@ -48,7 +48,7 @@ def attend(lib, ws=A, ws_bytes=1 << 40, **kw):
     (dict(eps=float("nan")), -1), (dict(head_dim=96), -2), (dict(head_dim=0), -2), (dict(half=0), -2),
     (dict(half=12), -2), (dict(half=40), -2), (dict(qkv=0), -1), (dict(cos=0), -1), (dict(pos=0), -1),
     (dict(q=0), -1), (dict(k=0), -1), (dict(qkv=A + 8), -1), (dict(cos=A + 4), -1), (dict(qw=A + 4), -1),
-    (dict(stride=3073), -1), (dict(qs=1028), -1), (dict(ks=1028), -1), (dict(limit=3), -1), (dict(rows=-1), -1),
+    (dict(stride=1537), -1), (dict(qs=516), -1), (dict(ks=516), -1), (dict(limit=3), -1), (dict(rows=-1), -1),
 ])
 def test_norm_refuses(lib, bad, status):
     assert norm(lib, **bad) == status
