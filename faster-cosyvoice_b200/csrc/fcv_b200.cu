@@ -678,6 +678,9 @@ int make_tmap_3d(CUtensorMap* m, const void* ptr, long d0, long d1, long d2, lon
   return FCV_OK;
 }
 
+// The row stride of a TMA tensor; a single row may have come with any.
+inline long tma_stride(long rows, long stride, long width) { return rows > 1 ? stride : width; }
+
 // Tensor-core kernel: whole items (list given) or the prefix parts.
 template <int D>
 int launch_sp_fa(const SpArgs& a, const SpPlan& p, int2* list, int* count, cudaStream_t s) {
@@ -688,16 +691,17 @@ int launch_sp_fa(const SpArgs& a, const SpPlan& p, int2* list, int* count, cudaS
   const int block = C::T * f.tile_tokens;
   const long cols = (long)a.Hkv * D;
   CUtensorMap tq, tpk, tpv, tk, tv, tv8, tv1;
-  FCV_TRY(make_tmap_3d(&tq, a.q, D, a.H, a.N, D, a.q_stride, a.G, f.tile_tokens));
+  FCV_TRY(make_tmap_3d(&tq, a.q, D, a.H, a.N, D, tma_stride(a.N, a.q_stride, (long)a.H * D), a.G, f.tile_tokens));
   // an absent tensor is stood in for by one query row that nothing reads unmasked
   const void* pk = a.P > 0 ? a.pk : a.q;
   const void* pv = a.P > 0 ? a.pv : a.q;
-  FCV_TRY(make_tmap_bf16(&tpk, pk, a.P > 0 ? a.P : 1, cols, a.P > 0 ? a.pk_stride : cols, kSfKeys));
-  FCV_TRY(make_tmap_bf16(&tpv, pv, a.P > 0 ? a.P : 1, cols, a.P > 0 ? a.pv_stride : cols, kSfKeys));
+  FCV_TRY(make_tmap_bf16(&tpk, pk, std::max(a.P, 1), cols, tma_stride(a.P, a.pk_stride, cols), kSfKeys));
+  FCV_TRY(make_tmap_bf16(&tpv, pv, std::max(a.P, 1), cols, tma_stride(a.P, a.pv_stride, cols), kSfKeys));
   const bool own = list && a.kv_rows > 0;
   const void* k = own ? a.k : a.q;
   const void* v = own ? a.v : a.q;
-  const long rows = own ? a.kv_rows : 1, ks = own ? a.k_stride : cols, vs = own ? a.v_stride : cols;
+  const long rows = own ? a.kv_rows : 1;
+  const long ks = tma_stride(rows, a.k_stride, cols), vs = tma_stride(rows, a.v_stride, cols);
   FCV_TRY(make_tmap_bf16(&tk, k, rows, cols, ks, kSfKeys));
   FCV_TRY(make_tmap_bf16(&tv, v, rows, cols, vs, kSfKeys));
   FCV_TRY(make_tmap_bf16(&tv8, v, rows, cols, vs, 8));
@@ -750,9 +754,9 @@ int launch_sp_stream(const SpArgs& a, cudaStream_t s) {
   using C = SpStream<D>;
   const long cols = (long)a.Hkv * D;
   CUtensorMap tq, tk, tv;
-  FCV_TRY(make_tmap_3d(&tq, a.q, D, a.H, a.N, D, a.q_stride, a.G, 16 / a.G));
-  FCV_TRY(make_tmap_bf16(&tk, a.k, a.kv_rows, cols, a.k_stride, kSpKeys));
-  FCV_TRY(make_tmap_bf16(&tv, a.v, a.kv_rows, cols, a.v_stride, kSpKeys));
+  FCV_TRY(make_tmap_3d(&tq, a.q, D, a.H, a.N, D, tma_stride(a.N, a.q_stride, (long)a.H * D), a.G, 16 / a.G));
+  FCV_TRY(make_tmap_bf16(&tk, a.k, a.kv_rows, cols, tma_stride(a.kv_rows, a.k_stride, cols), kSpKeys));
+  FCV_TRY(make_tmap_bf16(&tv, a.v, a.kv_rows, cols, tma_stride(a.kv_rows, a.v_stride, cols), kSpKeys));
   static bool attr[64] = {false};
   int dev = 0;
   cudaGetDevice(&dev);

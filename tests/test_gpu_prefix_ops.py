@@ -448,6 +448,13 @@ def test_expanded_rows():
                                         none, none)
     want = one.repeat_interleave(H // Hkv, 1).expand(300, -1, -1).double()
     assert ((got.double() - want).abs() <= 2 * 2.0 ** -8 * want.abs()).all()
+    # one query and one own key, each a row of stride 0, behind a long prefix
+    pre = torch.randn(5000, Hkv, D, generator=g, device=DEV).bfloat16()
+    row = torch.randn(H, D, generator=g, device=DEV).bfloat16()
+    key = torch.randn(Hkv, D, generator=g, device=DEV).bfloat16()
+    args = (pre, pre, torch.tensor([0, 1], dtype=torch.int32, device=DEV), none, none + 1)
+    got = ops().shared_prefix_attention(row.expand(1, -1, -1), key.expand(1, -1, -1), key.expand(1, -1, -1), *args)
+    assert torch.equal(got, ops().shared_prefix_attention(row[None].clone(), key[None].clone(), key[None].clone(), *args))
 
 
 @pytest.mark.parametrize("value", [float("nan"), float("inf")])
