@@ -1306,7 +1306,7 @@ int fcv_qk_norm_rope(const fcv_qk_norm* g, void* stream) {
   a.kv_limit = g->kv_limit;
   // A warp per token; tokens too few to give every SM eight warps share out their heads (one token of
   // 16/16 heads of 64: 2.2 us against 3.6).  More warps per token cost more than they hide: each reads
-  // the position, the tables and the weights again (96000 tokens: 1, 2, 3 warps 144, 156, 190 us).
+  // the position, the tables and the weights again (96000 tokens with 1, 2, 3 warps: 144, 156, 190 us).
   const int steps = (g->heads + g->kv_heads + 256 / g->head_dim - 1) / (256 / g->head_dim);
   a.warps_per_row = (int)std::max(1L, std::min((long)steps, 8L * num_sms() / g->N));
   cudaStream_t s = as_stream(stream);

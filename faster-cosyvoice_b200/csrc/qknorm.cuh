@@ -8,10 +8,10 @@
 // output is rounded once.
 //
 // Bound by memory: every value is read and written once.  On a B200 (copy: 6.54 TB/s): 96000 tokens
-// of 16/16 heads of 64 in bf16, 788 MB, 147 us (5.3 TB/s); 6577 tokens of 32/8 heads of 128 into
-// scattered cache rows, 164 MB, 34 us (4.8 TB/s); 20914 tokens of 16/16 heads of 64 in float32,
-// 343 MB, 56 us (6.1 TB/s).  Two, three and six steps in flight and three or four blocks on an SM
-// measure the same within 1 %.
+// of 16/16 heads of 64 in bf16, 788 MB, 140 us (5.6 TB/s); 6577 tokens of 32/8 heads of 128 into
+// scattered cache rows, 164 MB, 31 us (5.3 TB/s); 20914 tokens of 16/16 heads of 64 in float32,
+// 343 MB, 54.5 us (6.3 TB/s).  Two, three and six steps in flight and three or four blocks on an SM
+// measure the same within 1 %; a warp that loops over tokens, the next one's loads ahead, 147 us.
 #pragma once
 
 #include "fcv_common.cuh"
