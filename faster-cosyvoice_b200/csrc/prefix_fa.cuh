@@ -94,23 +94,31 @@ __global__ void __launch_bounds__(1024) sp_list_kernel(const SpArgs a, int block
   griddep_wait();
   griddep_launch();
   __shared__ int hist[1024], most, total;
+  __shared__ int2 lens[1024];  // queries and own keys of the first sequences; later ones are read each time
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
+  auto read = [&](int b, bool report) -> int2 {
+    const int c0 = a.cu[b], c1 = a.cu[b + 1];
+    int nq = c1 - c0;
+    const int nk = a.kv_lens ? a.kv_lens[b] : nq;
+    if (c0 < 0 || c1 < c0 || c1 > a.N) {
+      if (report) record_error(611);
+      nq = 0;
+    }
+    return make_int2(nq, nk);
+  };
+  for (int b = tid; b < a.B; b += 1024) {
+    const int2 s = read(b, true);
+    if (b < 1024) lens[b] = s;
+  }
   hist[tid] = 0;
   if (tid == 0) most = 1;
   __syncthreads();
   auto each = [&](auto f) {
     for (int b = warp; b < a.B; b += 32) {
-      SpSeq s;
-      const int c0 = a.cu[b], c1 = a.cu[b + 1];
-      s.nq = c1 - c0;
-      if (c0 < 0 || c1 < c0 || c1 > a.N) {
-        if (lane == 0) record_error(611);
-        s.nq = 0;
-      }
-      s.nk = a.kv_lens ? a.kv_lens[b] : s.nq;
-      for (int i = lane; (long)i * block < s.nq; i += 32) {
-        const int last = min((long)(i + 1) * block, (long)s.nq) - 1;
-        f(b, i, (sp_limit_at(a, s.nk, s.nk - s.nq + last) + kSfKeys - 1) / kSfKeys);
+      const int2 s = b < 1024 ? lens[b] : read(b, false);
+      for (int i = lane; (long)i * block < s.x; i += 32) {
+        const int last = min((long)(i + 1) * block, (long)s.x) - 1;
+        f(b, i, (sp_limit_at(a, s.y, s.y - s.x + last) + kSfKeys - 1) / kSfKeys);
       }
     }
   };

@@ -281,7 +281,8 @@ def shared_prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, p
 
     ``chunk``: 1 is causal, 0 shows every own key, c > 1 is the streaming mask of
     :func:`ragged_attention` over absolute positions (the prefix occupies positions 0 .. P - 1, the
-    queries are the last positions of their sequence).  ``scale`` defaults to head_dim ** -0.5.
+    queries are the last positions of their sequence).  ``scale`` (positive) defaults to
+    head_dim ** -0.5.
 
     Returns ``out`` (N, heads, head_dim); a query that sees no key gives zeros, rows of ``out``
     behind ``cu_seqlens[-1]`` are not written.  Row numbers are checked on the device
