@@ -8,10 +8,11 @@
 // items.  An item that lies inside one stretch leaves one part; an item that is cut leaves a part in
 // every stretch it meets, which sp_join_kernel finds by the same arithmetic.
 //
-// One block for each item and part, instead, loses a few microseconds at each start and end: 64
-// sequences of 1 to 1023 keys (8 key heads of 128, 118 MB) then took 45 us in one part each and 70 us
-// cut into four; the stretches take 33 us beside the prefix parts on 116 SMs, 3.6 TB/s; 256 sequences
-// (1.07 GB) on 100 SMs 225 us, 4.8 TB/s.  An SM takes in 59 GB/s at most through TMA.  Measured and not
+// One block for each item and part, instead, loses a few microseconds at each start and end: for 64
+// sequences of 1 to 1024 keys (8 key heads of 128, 134 MB) behind 4096 the call then took 61 us of device
+// time in one part each, 70 in two, 90 in four; it takes 43 us with the stretches, which run 34 to 35 us
+// on 108 SMs beside the prefix parts on 40, 3.9 TB/s.  256 sequences (1.07 GB) on 100 SMs: 225 us,
+// 4.7 TB/s.  18 CTAs alone took in 59 GB/s each.  Measured and not
 // kept: a fifth stage paid for by a join in two rounds (49 against 44 us), a group of warps for every
 // other item, and key heads outermost in the order (no change).
 #pragma once
