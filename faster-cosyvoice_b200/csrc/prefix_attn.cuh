@@ -734,6 +734,9 @@ __global__ void __launch_bounds__(256) sp_join_kernel(const SpArgs a) {
   }
   griddep_wait();
   griddep_launch();
+  // without own parts no kernel before this one has looked at the sequences
+  if (blockIdx.x == 0 && a.cuts == 0 && a.own_parts == 0)
+    for (int i = threadIdx.x; i < a.B; i += blockDim.x) sp_sequence(a, i, true);
   if (token >= a.N || token < begin || token >= end) return;  // rows behind the last sequence stay
   // own parts: all of them, or (cuts) one in the row's own place or one in each stretch that the item meets
   int own = a.own_parts, first = -1, prefix_parts = a.prefix_parts;

@@ -626,3 +626,36 @@ def test_two_calls_at_once_on_two_streams():
             got.append((o.shared_prefix_attention(**b), rb))
     torch.cuda.synchronize()
     assert all(torch.equal(x, y) for x, y in got)
+
+
+@pytest.mark.parametrize("H,Hkv,D,P", [(32, 8, 128, 8000), (32, 8, 128, 3000), (16, 4, 64, 6000)])
+def test_no_own_keys_at_all_behind_a_long_prefix(H, Hkv, D, P):
+    """Key tensors without rows leave the parts of the prefix alone; offsets and lengths that are out of
+    range are still reported."""
+    from fcv_b200 import _lib
+
+    B = 64
+    args, base, _ = attention_inputs([1] * B, [0] * B, P, H, Hkv, D, torch.bfloat16, 91, poison=False)
+    args["k"], args["v"] = args["k"][:0], args["v"][:0]
+    args["kv_base"].zero_()
+    args["kv_lens"].zero_()
+    count = _lib.lib().fcv_launch_count
+    before = count()
+    good = ops().shared_prefix_attention(**args)
+    assert count() - before == 2  # the parts of the prefix and their join
+    assert ops().device_error() == 0
+    ref = attention_ref(args["q"], args["k"], args["v"], args["prefix_k"], args["prefix_v"], [1] * B, [0] * B, [0] * B, 1,
+                        D ** -0.5)
+    check_attention(good, ref, P)
+    lens = args["kv_lens"].clone()
+    lens[5] = 3
+    assert torch.equal(ops().shared_prefix_attention(**dict(args, kv_lens=lens)), good)
+    assert ops().device_error() == 612
+    cu = args["cu_seqlens"].clone()
+    cu[-1] = B + 2
+    got = ops().shared_prefix_attention(**dict(args, cu_seqlens=cu))
+    assert ops().device_error() == 611
+    assert torch.equal(got[:B - 1], good[:B - 1])
+    cu[-1], cu[-2] = B, B - 3
+    ops().shared_prefix_attention(**dict(args, cu_seqlens=cu))
+    assert ops().device_error() == 611
