@@ -550,7 +550,9 @@ SpPlan sp_plan(const fcv_prefix_attention& g) {
                       apart(kv_rows, g.v_stride, (long)Hkv * D);
   p.prefix_rows = rows <= 16 ? 16 : 64;
   p.own_rows = own <= 16 ? 16 : 64;
-  const bool stream = tensor && G <= 16 && own <= 16;
+  // without own keys at all the prefix parts have every SM, and the join finds no own part
+  const bool none = tensor && P > 0 && kv_rows == 0;
+  const bool stream = tensor && G <= 16 && own <= 16 && !none;
   const int d = D == 64 ? 0 : 1, r = p.own_rows == 16 ? 0 : 1;
   const double all = (double)(tiles + own_tiles), own_blocks = (double)B * Hkv * ((own + p.own_rows - 1) / p.own_rows);
   const double load = own_blocks / sms;  // blocks of sp_pieces_kernel on an SM
@@ -572,8 +574,9 @@ SpPlan sp_plan(const fcv_prefix_attention& g) {
       fa_parts = std::min(fa_parts, std::ceil(blocks * n / sms) * ((tiles + n - 1) / n * kFull[d] + 6) + 0.1 * n);
     if (P == 0) fa_parts = 0;
     const double units = (double)B * Hkv * (own_tiles + kSsItem);
-    const double own_us = stream ? units * std::max((d ? 0.66 : 0.33) / sms, d ? 0.0056 : 0.0028)
-                                 : std::max(own_tiles * kAlone[d][r], load * (own_tiles * kAmong[d][r] + 0.6)) + 3;
+    const double own_us = none     ? 0
+                          : stream ? units * std::max((d ? 0.66 : 0.33) / sms, d ? 0.0056 : 0.0028)
+                                   : std::max(own_tiles * kAlone[d][r], load * (own_tiles * kAmong[d][r] + 0.6)) + 3;
     parts_us = 10 + std::max(fa_parts, own_us) + 0.35 * std::min(fa_parts, own_us) + (double)N * H * D * 16 / 2.5e6;
   } else {
     // fp32, in tile steps of an SM's two blocks (5 and 9 us); the choice is 0.3 % slower than the better way
@@ -636,6 +639,18 @@ SpPlan sp_plan(const fcv_prefix_attention& g) {
     }
     for (int i = 0; i < p.split.n; ++i) p.prefix_parts = std::max(p.prefix_parts, p.split.parts[i]);
     p.fa_ctas = (int)sms;
+  } else if (p.fa_prefix && none) {
+    // Even waves of parts, with the join's traffic; a ninth of the SMs is left to the join of the call
+    // before (16 streams of 32/8 heads of 128 behind 16000 keys, calls one after another: 31 us in 128
+    // items, 35 in 144).  Chosen as beside own keys, or on the SMs left beside them, 14 shapes took 0.95 to
+    // 1.33 times as long (256 streams behind 8000 keys, 32/8 heads of 128: 65 us against 55).
+    p.fa_ctas = (int)sms;
+    double best = 0;
+    for (long n = 1; n <= 24 && (n == 1 || (n - 1) * 4 < tiles); ++n) {
+      const double waves = std::ceil((double)(p.prefix_blocks * Hkv * n) / (sms - sms / 9));
+      const double us = waves * ((tiles + n - 1) / n * kFull[d] + 6) + n * (double)N * H * D * 8 / 2.5e6;
+      if (best == 0 || us < best) best = us, p.prefix_parts = (int)n;
+    }
   } else if (p.fa_prefix) {
     p.fa_ctas = (int)sms;
     // waves of equal parts: the fewest tile steps on the busiest SM, a part costing two more
@@ -650,7 +665,9 @@ SpPlan sp_plan(const fcv_prefix_attention& g) {
     const long blocks = p.prefix_blocks * Hkv;
     p.prefix_parts = (int)std::max(1L, std::min(std::min(64L, tiles), (2 * sms + blocks - 1) / blocks));
   }
-  if (stream) {
+  if (none) {
+    p.own_parts = 0;
+  } else if (stream) {
     p.own_parts = 1;
     p.cuts = (int)sms;
   } else {
@@ -1413,12 +1430,6 @@ int fcv_shared_prefix_attention(const fcv_prefix_attention* g, void* workspace, 
       a.split.n = 0;
       break;
     }
-  }
-  if (kv_rows == 0 && p.cuts) {  // no own keys at all: nothing to stream, and the join finds no own part
-    a.cuts = 0;
-    a.own_parts = 0;
-    if (a.split.n) a.prefix_parts = a.split.parts[a.split.n - 1];
-    a.split.n = 0;
   }
   const size_t rows = (size_t)(p.prefix_parts + p.own_parts) * N * heads;
   if (a.cuts) {

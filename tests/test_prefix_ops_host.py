@@ -85,6 +85,17 @@ def test_workspace_is_sized_on_the_host(lib):
     assert size(N=64, B=64, heads=32, kv_heads=8, head_dim=128, P=4096, dtype=0) >= 2 * 64 * 32 * (128 * 4 + 8)
 
 
+@pytest.mark.parametrize("P", [3000, 8000, 16384])
+def test_key_tensors_without_rows_leave_every_sm_to_the_prefix(lib, P):
+    """The workspace is the parts of the prefix alone: no place for an own part, no stretches of own keys
+    that would take a share of the SMs."""
+    shape = dict(N=64, B=64, heads=32, kv_heads=8, head_dim=128, P=P, qs=4096, os=4096)
+    part = 64 * 32 * (128 * 4 + 8)
+    size = lib.fcv_shared_prefix_workspace_bytes(attention(rows=0, **shape))
+    assert size > 0 and size % part == 0
+    assert lib.fcv_shared_prefix_workspace_bytes(attention(rows=64 * 64, **shape)) % part != 0
+
+
 @pytest.mark.parametrize("name", ["fcv_qk_norm", "fcv_prefix_attention"])
 def test_packed_arguments_have_the_layout_of_the_header(name):
     """The format strings against the structures that the header declares, field by field."""
