@@ -659,3 +659,29 @@ def test_no_own_keys_at_all_behind_a_long_prefix(H, Hkv, D, P):
     cu[-1], cu[-2] = B, B - 3
     ops().shared_prefix_attention(**dict(args, cu_seqlens=cu))
     assert ops().device_error() == 611
+
+
+def way_inputs(way, dtype, extra=4):
+    """Inputs of a way of cutting, with the own keys named by offsets, and a sequence without queries at
+    the end; `extra` rows of q lie behind the last sequence."""
+    (q_lens, past, P, H, Hkv, D), _ = WAYS[way]
+    if dtype == torch.float32:
+        q_lens, past, P = q_lens[:8], past and past[:8], min(P, 900)
+    q_lens, past = q_lens + [0], past and past + [0]
+    args, base, kv_lens = attention_inputs(q_lens, past, P, H, Hkv, D, dtype, 81, extra=extra, poison=False)
+    t = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    args["kv_base"], args["kv_lens"] = t(base), t(kv_lens)
+    return args, q_lens, base, kv_lens
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("way", list(WAYS))
+def test_keys_out_of_range_of_a_sequence_without_queries_are_reported(way, dtype):
+    args, q_lens, base, kv_lens = way_inputs(way, dtype)
+    good = ops().shared_prefix_attention(**args)
+    assert ops().device_error() == 0
+    args["kv_base"][-1], args["kv_lens"][-1] = args["k"].shape[0] - 1, 2
+    got = ops().shared_prefix_attention(**args)
+    assert ops().device_error() == 612
+    used = sum(q_lens)
+    assert torch.equal(got[:used], good[:used])
