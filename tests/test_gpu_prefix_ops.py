@@ -685,3 +685,51 @@ def test_keys_out_of_range_of_a_sequence_without_queries_are_reported(way, dtype
     assert ops().device_error() == 612
     used = sum(q_lens)
     assert torch.equal(got[:used], good[:used])
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("way", list(WAYS))
+def test_bad_rows_in_every_way_of_cutting(way, dtype):
+    """Own keys out of range cost their sequence its own keys and nothing else; offsets out of order or
+    range spare the rows that lie outside the refused pairs; rows behind the last sequence stay."""
+    args, q_lens, base, kv_lens = way_inputs(way, dtype)
+    P, D, used, N, rows = args["prefix_k"].shape[0], args["q"].shape[2], sum(q_lens), args["q"].shape[0], args["k"].shape[0]
+    j = next(b for b in range(1, len(q_lens)) if q_lens[b] > 0 and kv_lens[b] > 1)
+    inputs = [args[n] for n in ("q", "k", "v", "prefix_k", "prefix_v")]
+    full = [x[:used] for x in attention_ref(*inputs, q_lens, base, kv_lens, 1, D ** -0.5)]
+    start = sum(q_lens[:j])
+    alone = attention_ref(inputs[0][start:], *inputs[1:], [q_lens[j]], [0], [0], 1, D ** -0.5)
+    without = [x.clone() for x in full]
+    for x, y in zip(without, alone):
+        x[start:start + q_lens[j]] = y[:q_lens[j]]
+
+    def call(error, **change):
+        out = torch.full((N,) + tuple(args["q"].shape[1:]), 7.0, dtype=dtype, device=DEV)
+        ops().shared_prefix_attention(**{**args, **change}, out=out)
+        assert ops().device_error() == error
+        return out
+
+    for name, value in (("kv_base", rows), ("kv_base", rows - 1), ("kv_base", -4), ("kv_lens", -5),
+                        ("kv_lens", rows + 1)):
+        bad = args[name].clone()
+        bad[j] = value
+        out = call(612, **{name: bad})
+        check_attention(out[:used], without, P + max(kv_lens))
+        assert (out[used:] == 7).all()
+    cu = args["cu_seqlens"]
+
+    def offsets(at, value, spared, behind=True):
+        bad = cu.clone()
+        bad[at] = value
+        out = call(611, cu_seqlens=bad)
+        keep = torch.ones(used, dtype=torch.bool, device=DEV)
+        keep[spared[0]:spared[1]] = False
+        check_attention(out[:used][keep], [x[keep] for x in full], P + max(kv_lens))
+        assert not behind or (out[used:] == 7).all()
+
+    offsets(len(q_lens), N + 3, (used, used), behind=False)  # the last sequence leaves the rows
+    offsets(0, -1, (0, q_lens[0]))
+    low = int(cu[j]) - 1
+    offsets(j + 1, low, (low, int(cu[j + 2]) if j + 2 < len(cu) else used))  # an offset that runs back
+    out = call(0)
+    check_attention(out[:used], full, P + max(kv_lens))
