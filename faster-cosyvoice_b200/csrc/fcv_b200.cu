@@ -1295,7 +1295,9 @@ int fcv_qk_norm_rope(const fcv_qk_norm* g, void* stream) {
                        reinterpret_cast<uintptr_t>(g->k_out) | reinterpret_cast<uintptr_t>(g->v_out) |
                        reinterpret_cast<uintptr_t>(g->rope_cos) | reinterpret_cast<uintptr_t>(g->rope_sin) |
                        reinterpret_cast<uintptr_t>(g->q_weight) | reinterpret_cast<uintptr_t>(g->k_weight);
-  if ((at & 15) || (((g->row_stride | g->q_stride | g->k_stride | g->v_stride) * es) & 15))
+  // the stride of a single row is never used
+  const long strides = (g->N > 1 ? g->row_stride | g->q_stride : 0) | (g->kv_limit > 1 ? g->k_stride | g->v_stride : 0);
+  if ((at & 15) || ((strides * es) & 15))
     return fail(FCV_EINVAL, "fcv_qk_norm_rope: rows, weights and tables must be 16-byte aligned");
   if (!g->kv_rows && g->kv_limit < g->N)
     return fail(FCV_EINVAL, "fcv_qk_norm_rope: %d rows into %ld", g->N, g->kv_limit);
@@ -1356,11 +1358,12 @@ int fcv_shared_prefix_attention(const fcv_prefix_attention* g, void* workspace, 
       (P > 0 && (!g->prefix_k || !g->prefix_v)) || (!g->kv_base != !g->kv_lens))
     return fail(FCV_EINVAL, "fcv_shared_prefix_attention: null pointer");
   const long es = (long)dsize(g->dtype);
-  const uintptr_t at = reinterpret_cast<uintptr_t>(g->q) | reinterpret_cast<uintptr_t>(g->k) |
-                       reinterpret_cast<uintptr_t>(g->v) | reinterpret_cast<uintptr_t>(g->prefix_k) |
-                       reinterpret_cast<uintptr_t>(g->prefix_v) | reinterpret_cast<uintptr_t>(g->out);
-  const long strides = g->q_stride | g->k_stride | g->v_stride | g->prefix_k_stride | g->prefix_v_stride |
-                       g->out_stride;
+  // the address of no rows and the stride of a single row are never used
+  uintptr_t at = reinterpret_cast<uintptr_t>(g->q) | reinterpret_cast<uintptr_t>(g->out);
+  if (kv_rows > 0) at |= reinterpret_cast<uintptr_t>(g->k) | reinterpret_cast<uintptr_t>(g->v);
+  if (P > 0) at |= reinterpret_cast<uintptr_t>(g->prefix_k) | reinterpret_cast<uintptr_t>(g->prefix_v);
+  const long strides = (N > 1 ? g->q_stride | g->out_stride : 0) | (kv_rows > 1 ? g->k_stride | g->v_stride : 0) |
+                       (P > 1 ? g->prefix_k_stride | g->prefix_v_stride : 0);
   if ((at & 15) || ((strides * es) & 15))
     return fail(FCV_EINVAL, "fcv_shared_prefix_attention: rows must be 16-byte aligned");
   if (P > 0x7fffff00 || kv_rows > 0x7fffff00L)  // row numbers of a tile past the last row stay 32-bit

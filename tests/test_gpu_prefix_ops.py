@@ -733,3 +733,33 @@ def test_bad_rows_in_every_way_of_cutting(way, dtype):
     offsets(j + 1, low, (low, int(cu[j + 2]) if j + 2 < len(cu) else used))  # an offset that runs back
     out = call(0)
     check_attention(out[:used], full, P + max(kv_lens))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("P,H,Hkv", [(1, 4, 2), (1, 130, 1), (5000, 16, 4)])
+def test_single_rows_of_odd_strides(dtype, P, H, Hkv):
+    """A row cut out of a buffer of odd width: its stride is never used."""
+    D = 64
+    odd = lambda n, h, seed: torch.randn(2 * (h * D + 3), generator=gen(seed), device=DEV).to(dtype).as_strided(  # noqa: E731
+        (n, h, D), (h * D + 3, D, 1))
+    q, k, v = odd(1, H, 1), odd(1, Hkv, 2), odd(1, Hkv, 3)
+    if P == 1:
+        pk, pv = odd(1, Hkv, 4), odd(1, Hkv, 5)
+    else:
+        pk, pv = (torch.randn(P, Hkv, D, generator=gen(s), device=DEV).to(dtype) for s in (4, 5))
+    t = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    out = odd(1, H, 6)
+    got = ops().shared_prefix_attention(q, k, v, pk, pv, t([0, 1]), t([0]), t([1]), out=out)
+    assert got is out
+    check_attention(got, attention_ref(q, k, v, pk, pv, [1], [0], [1], 1, D ** -0.5), P + 1)
+    # the norm of one such row, into a cache of one
+    width = (H + 2 * Hkv) * D
+    qkv, qw, kw, cos, sin, pos = norm_inputs(1, H, Hkv, D, 32, dtype, 7)
+    row = torch.empty(width + 3, dtype=dtype, device=DEV).as_strided((1, width), (width + 3, 1)).copy_(qkv)
+    cache = torch.empty(2 * Hkv * D + 3, dtype=dtype, device=DEV).as_strided((1, 2 * Hkv * D), (2 * Hkv * D + 3, 1))
+    q0, k0 = ops().qk_norm_rope(qkv, qw, kw, cos, sin, pos, H, Hkv)
+    q1, _ = ops().qk_norm_rope(row, qw, kw, cos, sin, pos, H, Hkv, kv_cache=cache, kv_rows=t([0]))
+    assert torch.equal(q1, q0) and torch.equal(cache[:, :Hkv * D], k0.flatten(1))
+    assert torch.equal(cache[:, Hkv * D:], qkv[:, (H + Hkv) * D:])
+    q2, k2 = ops().qk_norm_rope(row, qw, kw, cos, sin, pos, H, Hkv, inplace=True)
+    assert torch.equal(q2, q0) and torch.equal(k2, k0)

@@ -69,6 +69,19 @@ def test_attention_refuses(lib, bad, status):
     assert b"fcv_shared_prefix_attention" in lib.fcv_last_error()
 
 
+@pytest.mark.parametrize("kw", [
+    dict(N=1, B=1, qs=1027, os=1029), dict(rows=1, ks=2049, vs=2051), dict(P=1, pks=2049, pvs=2051),
+    dict(rows=0, k=A + 2, v=A + 4, ks=2049), dict(P=0, pk=A + 2, pv=A + 4, pks=2049),
+])
+def test_single_rows_have_any_stride_and_no_rows_any_address(lib, kw):
+    """Such a call passes the check of alignment and stops at the workspace, which is refused last."""
+    assert attend(lib, ws=A + 4, dtype=0, **kw) == -1
+    assert b"workspace" in lib.fcv_last_error()
+    if "rows" not in kw and "P" not in kw:  # the norm: its last check is of the rows of its output
+        assert norm(lib, N=1, stride=1537, qs=513, ks=513, limit=0) == -1
+        assert b"1 rows into 0" in lib.fcv_last_error()
+
+
 def test_empty_calls_return_before_any_launch(lib):
     assert lib.fcv_qk_norm_rope(None, None) == -1 and lib.fcv_shared_prefix_attention(None, None, 0, None) == -1
     assert norm(lib, N=0, qkv=0) == 0
