@@ -1351,8 +1351,8 @@ int fcv_shared_prefix_attention(const fcv_prefix_attention* g, void* workspace, 
     return fail(FCV_EINVAL, "fcv_shared_prefix_attention: %d heads over %d key heads", heads, kv_heads);
   if (head_dim != 64 && head_dim != 128)
     return fail(FCV_EUNSUPPORTED, "fcv_shared_prefix_attention: head_dim must be 64 or 128 (got %d)", head_dim);
-  if (!(g->scale > 0.f) || g->scale > 3.0e38f)
-    return fail(FCV_EINVAL, "fcv_shared_prefix_attention: scale must be positive");
+  if (!(g->scale > 0.f) || !std::isfinite(g->scale * kLog2e))  // the kernels scale in log2 units
+    return fail(FCV_EINVAL, "fcv_shared_prefix_attention: scale must be positive and at most 2.3e38");
   if (N == 0 || B == 0) return FCV_OK;
   if (!g->q || !g->cu_seqlens || !g->out || (kv_rows > 0 && (!g->k || !g->v)) ||
       (P > 0 && (!g->prefix_k || !g->prefix_v)) || (!g->kv_base != !g->kv_lens))

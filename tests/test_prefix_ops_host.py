@@ -82,6 +82,12 @@ def test_single_rows_have_any_stride_and_no_rows_any_address(lib, kw):
         assert b"1 rows into 0" in lib.fcv_last_error()
 
 
+def test_a_scale_that_overflows_in_log2_units_is_refused(lib):
+    """The kernels multiply by scale * log2(e), which has to be finite (2.9e38 * 1.44 > 3.4e38)."""
+    assert attend(lib, scale=2.9e38, ws=A + 4) == -1 and b"scale" in lib.fcv_last_error()
+    assert attend(lib, scale=2.3e38, ws=A + 4) == -1 and b"workspace" in lib.fcv_last_error()
+
+
 def test_empty_calls_return_before_any_launch(lib):
     assert lib.fcv_qk_norm_rope(None, None) == -1 and lib.fcv_shared_prefix_attention(None, None, 0, None) == -1
     assert norm(lib, N=0, qkv=0) == 0
