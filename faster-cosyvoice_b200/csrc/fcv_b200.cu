@@ -579,10 +579,12 @@ SpPlan sp_plan(const fcv_prefix_attention& g) {
                                    : std::max(own_tiles * kAlone[d][r], load * (own_tiles * kAmong[d][r] + 0.6)) + 3;
     parts_us = 10 + std::max(fa_parts, own_us) + 0.35 * std::min(fa_parts, own_us) + (double)N * H * D * 16 / 2.5e6;
   } else {
-    // fp32, in tile steps of an SM's two blocks (5 and 9 us); the choice is 0.3 % slower than the better way
-    // over the same shapes
-    whole_us = (load / 2 + 0.4) * all;
-    parts_us = ((rows + p.prefix_rows - 1) / p.prefix_rows * Hkv * tiles + own_blocks * own_tiles) / (2.0 * sms) + 1.5 +
+    // fp32, in tile steps (5 and 9 us) of the blocks that an SM holds by their shared memory: two for heads
+    // of 64, one for heads of 128.  Over the same shapes the choice is on average 0.1 and 0.2 % slower than the
+    // better way, at worst 1.10 and 1.20 times (with two blocks for heads of 128: 0.4 %, 1.31 times).
+    const double held = d ? 1 : 2;
+    whole_us = (load / held + 0.4) * all;
+    parts_us = ((rows + p.prefix_rows - 1) / p.prefix_rows * Hkv * tiles + own_blocks * own_tiles) / (held * sms) + 1.5 +
                (double)N * H * D * 16 / 2.5e6 / (d ? 9 : 5);
     if (load < 1) whole_us = all;
   }
@@ -661,7 +663,8 @@ SpPlan sp_plan(const fcv_prefix_attention& g) {
       if (best == 0 || cost < best) best = cost, p.prefix_parts = n;
     }
   } else if (P > 0) {
-    // enough blocks for two on every SM
+    // two blocks for every SM; heads of 128 in fp32 run them one after another, and one block for every
+    // SM measures the same on average (1.00 over 164 shapes, 0.73 to 1.50)
     const long blocks = p.prefix_blocks * Hkv;
     p.prefix_parts = (int)std::max(1L, std::min(std::min(64L, tiles), (2 * sms + blocks - 1) / blocks));
   }

@@ -104,6 +104,14 @@ def test_workspace_is_sized_on_the_host(lib):
     assert size(N=64, B=64, heads=32, kv_heads=8, head_dim=128, P=4096, dtype=0) >= 2 * 64 * 32 * (128 * 4 + 8)
 
 
+def test_float32_heads_of_128_are_planned_at_one_block_an_sm(lib):
+    """128 sequences of 5 to 8 queries behind 200 keys, 8/1 heads of 128: whole blocks take 60 us and parts
+    79; whole blocks need no workspace.  Behind 2000 keys parts are faster."""
+    shape = dict(N=851, B=128, heads=8, kv_heads=1, head_dim=128, rows=128 * 128, qs=1024, os=1024, dtype=0)
+    assert lib.fcv_shared_prefix_workspace_bytes(attention(P=200, **shape)) == 0
+    assert lib.fcv_shared_prefix_workspace_bytes(attention(P=2000, **shape)) > 0
+
+
 @pytest.mark.parametrize("P", [3000, 8000, 16384])
 def test_key_tensors_without_rows_leave_every_sm_to_the_prefix(lib, P):
     """The workspace is the parts of the prefix alone: no place for an own part, no stretches of own keys
