@@ -561,13 +561,17 @@ SpPlan sp_plan(const fcv_prefix_attention& g) {
   // a tile step of a tensor-core item by its query tiles in use; in full (prefix parts)
   static const double kStep[2][3] = {{0.78, 1.0, 1.25}, {0.86, 1.1, 1.1}}, kFull[2] = {1.25, 1.1};
   double fa_us = 1e30, whole_us, parts_us = 1e30;
+  // parts that make two blocks for every SM out of `blocks`; heads of 128 in fp32 run them one after
+  // another, and one block for every SM measures the same on average (1.00 over 164 shapes, 0.73 to 1.50)
+  auto two_each = [&](long blocks, long most) { return std::max(1L, std::min(most, (2 * sms + blocks - 1) / blocks)); };
+  if (bf)
+    whole_us = 5.5 + 2 * d + (load <= 1 ? all * kAlone[d][r]
+                                        : std::max(all * kAlone[d][r], (load + 0.5) * all * kAmong[d][r]) + 0.3 * load);
   if (tensor) {
     const long used = std::min((long)(D == 64 ? 3 : 2), (q_len + tile - 1) / tile);
     const double items = (double)std::min((long)B, N) * ((q_len + block - 1) / block) * Hkv;
     const double waves = items <= sms ? 1.0 : items / sms + 0.3;
     fa_us = 10.5 + waves * (all * kStep[d][used - 1] + 1.5);
-    whole_us = 5.5 + 2 * d + (load <= 1 ? all * kAlone[d][r]
-                                        : std::max(all * kAlone[d][r], (load + 0.5) * all * kAmong[d][r]) + 0.3 * load);
     const double blocks = (double)((N + block - 1) / block) * Hkv;
     double fa_parts = 1e30;
     for (long n = 1; n <= 24 && (n == 1 || (n - 1) * 4 < tiles); ++n)
@@ -578,6 +582,20 @@ SpPlan sp_plan(const fcv_prefix_attention& g) {
                           : stream ? units * std::max((d ? 0.66 : 0.33) / sms, d ? 0.0056 : 0.0028)
                                    : std::max(own_tiles * kAlone[d][r], load * (own_tiles * kAmong[d][r] + 0.6)) + 3;
     parts_us = 10 + std::max(fa_parts, own_us) + 0.35 * std::min(fa_parts, own_us) + (double)N * H * D * 16 / 2.5e6;
+  } else if (bf) {
+    // all in sp_pieces_kernel, and the join; short parts stay empty.  Over 422 shapes, those above and 130/1
+    // heads of 64, the choice is on average 1.6 % slower than the better way, at worst 1.85 times (4 sequences
+    // of about 160 queries behind 200 keys, 8/1 heads of 128: 69 us whole, 38 in parts).
+    constexpr long least = sp_least<bf16>();
+    const long blocks = (rows + p.prefix_rows - 1) / p.prefix_rows * Hkv;
+    const long pre = P > 0 ? std::min(two_each(blocks, std::min(64L, tiles)), (tiles + least - 1) / least) : 0;
+    const long mine = std::min(two_each((long)own_blocks, 16), (own_tiles + least - 1) / least);
+    const int rp = p.prefix_rows == 16 ? 0 : 1;
+    const double longest = std::max(pre ? (tiles + pre - 1) / pre * kAlone[d][rp] : 0.0,
+                                    (own_tiles + mine - 1) / mine * kAlone[d][r]);
+    const double among = (blocks * (tiles * kAmong[d][rp] + 0.5 * pre) +
+                          own_blocks * (own_tiles * kAmong[d][r] + 0.5 * mine)) / sms;
+    parts_us = 7.5 + 2 * d + std::max(longest, among) + (double)(pre + mine) * N * H * D * 8 / 2.5e6;
   } else {
     // fp32, in tile steps (5 and 9 us) of the blocks that an SM holds by their shared memory: two for heads
     // of 64, one for heads of 128.  Over the same shapes the choice is on average 0.1 and 0.2 % slower than the
@@ -663,10 +681,7 @@ SpPlan sp_plan(const fcv_prefix_attention& g) {
       if (best == 0 || cost < best) best = cost, p.prefix_parts = n;
     }
   } else if (P > 0) {
-    // two blocks for every SM; heads of 128 in fp32 run them one after another, and one block for every
-    // SM measures the same on average (1.00 over 164 shapes, 0.73 to 1.50)
-    const long blocks = p.prefix_blocks * Hkv;
-    p.prefix_parts = (int)std::max(1L, std::min(std::min(64L, tiles), (2 * sms + blocks - 1) / blocks));
+    p.prefix_parts = (int)two_each(p.prefix_blocks * Hkv, std::min(64L, tiles));
   }
   if (none) {
     p.own_parts = 0;
@@ -674,7 +689,7 @@ SpPlan sp_plan(const fcv_prefix_attention& g) {
     p.own_parts = 1;
     p.cuts = (int)sms;
   } else {
-    p.own_parts = (int)std::max(1L, std::min(16L, (2 * sms + (long)own_blocks - 1) / (long)own_blocks));
+    p.own_parts = (int)two_each((long)own_blocks, 16);
   }
   p.part_bytes = (size_t)(p.prefix_parts + p.own_parts) * N * H * (D * sizeof(float) + sizeof(float2));
   p.part_bytes = (p.part_bytes + 15) / 16 * 16;

@@ -112,6 +112,14 @@ def test_float32_heads_of_128_are_planned_at_one_block_an_sm(lib):
     assert lib.fcv_shared_prefix_workspace_bytes(attention(P=2000, **shape)) > 0
 
 
+def test_bf16_off_the_tensor_cores_is_planned_by_its_own_steps(lib):
+    """130 heads to a key head: 191 queries of one sequence behind 200 keys take 41 us in whole blocks, which
+    need no workspace, and 199 in parts; one query behind 8000 keys is cut into parts."""
+    shape = dict(heads=130, kv_heads=1, head_dim=64, B=1, qs=8320, os=8320)
+    assert lib.fcv_shared_prefix_workspace_bytes(attention(N=191, P=200, rows=1408, **shape)) == 0
+    assert lib.fcv_shared_prefix_workspace_bytes(attention(N=1, P=8000, rows=64, **shape)) > 0
+
+
 @pytest.mark.parametrize("P", [3000, 8000, 16384])
 def test_key_tensors_without_rows_leave_every_sm_to_the_prefix(lib, P):
     """The workspace is the parts of the prefix alone: no place for an own part, no stretches of own keys
