@@ -42,6 +42,15 @@ __device__ __forceinline__ uint32_t smem_u32(const void* p) {
 // Both are no-ops for a launch without the programmatic-serialization attribute.
 // Because every CTA waits before it exits, a kernel's completion implies the
 // completion of all kernels before it on the stream.
+//
+// Exceptions, in the shared-prefix attention: sp_stream_kernel and sp_pieces_kernel with `beside`
+// read the caller's tensors and write the workspace before their wait, which stands at their end, and
+// sp_join_kernel reads the caller's cu_seqlens, kv_base and kv_lens before its own.  What makes that
+// right is that a kernel starts only when every CTA of the one launched before it has called
+// griddep_launch() or left: sp_fa_kernel, and sp_stream_kernel and sp_pieces_kernel without `beside`,
+// call it only after their griddep_wait(), so whatever was on the stream before the attention call is
+// complete by then (beside sp_fa_kernel, because that one had waited).  So those kernels must not
+// launch before they wait, and no kernel that does may come between them.
 __device__ __forceinline__ void griddep_wait() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void griddep_launch() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 

@@ -180,7 +180,7 @@ __global__ void __launch_bounds__(SpFa<D>::THREADS, 1)
   int prefix_items = f.prefix_items, prefix_parts = A.prefix_parts, prefix_ctas = gridDim.x;
   if (A.split.n > 0) {
     griddep_wait();
-    griddep_launch();
+    griddep_launch();  // only after the wait: the kernels behind this one rely on it (fcv_common.cuh)
     // this kernel's share of the SMs follows from the own keys
     __shared__ unsigned long long units;
     if (threadIdx.x == 0) units = 0;
@@ -241,7 +241,7 @@ __global__ void __launch_bounds__(SpFa<D>::THREADS, 1)
   const uint32_t tmem = *tmem_slot;
   if (A.split.n == 0) {
     griddep_wait();
-    griddep_launch();
+    griddep_launch();  // only after the wait, as above
   }
 
   if (warp >= C::PRODUCER) {
