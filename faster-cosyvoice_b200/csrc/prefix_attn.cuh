@@ -7,11 +7,13 @@
 // over the whole prefix and the own keys j with (P + j) / chunk <= (P + nk - nq + i) / chunk
 // (integer division; chunk 0: every own key).  A row that sees no key is zero.
 //
-// Query rows are stacked over the heads of a key head: stacked row R = token * G + g.  The prefix
-// belongs to no sequence, so its products run over stacked rows of the whole batch -- each prefix
-// key is read once for 64 rows, not once for every sequence -- and the own keys run per sequence.
+// Query rows are stacked over the heads of a key head: stacked row R = token * G + g.  Cut into parts,
+// the prefix, which belongs to no sequence, takes stacked rows of the whole batch -- each of its keys
+// is read once for 64 rows or more, not once for every sequence -- and the own keys run per sequence.
 // Each piece of keys leaves a running maximum, sum and unnormalised output in float32; a second
-// kernel joins the pieces of a row.
+// kernel joins the pieces of a row.  Whole, a block takes rows of one sequence through the prefix and
+// its own keys in one go, so every sequence reads the prefix again and nothing is joined; short
+// prefixes and long queries are faster that way.
 //
 // This file has the kernel for few rows in bf16 (mma.sync: 16 to 64 rows to a block, bound by the
 // latency of a key tile, 0.43 us for 16 rows of 64 values, 0.74 us of 128) and for all of float32 (CUDA

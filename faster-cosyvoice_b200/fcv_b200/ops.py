@@ -201,8 +201,10 @@ def qk_norm_rope(qkv: torch.Tensor, q_weight: torch.Tensor | None, k_weight: tor
     Returns ``(q, k)``: (N, heads, head_dim) and (N, kv_heads, head_dim), new tensors or, with
     ``inplace``, views of ``qkv``, whose query and key columns are rewritten.  With ``kv_cache``
     (rows, 2 kv_heads head_dim) of [K | V] and int32 ``kv_rows`` (N) the keys and the values go to
-    those cache rows instead and ``(q, kv_cache)`` is returned; a negative row stores nothing (a
-    padding token), and the others must differ from one another.
+    those cache rows instead and ``(q, kv_cache)`` is returned (with ``inplace`` the query columns of
+    ``qkv`` are rewritten, its key and value columns stay); a negative row stores nothing (a padding
+    token), and the others must differ from one another.  Forward only: the outputs carry no
+    gradient.
 
     A position outside the tables or a row outside the cache is not accessed: the token (its keys
     and values) stays unwritten and :func:`device_error` reports 601 (602)."""
@@ -273,7 +275,8 @@ def shared_prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, p
 
     ``q``: (N, heads, head_dim) packed query rows, sequence b at ``cu_seqlens[b] ..
     cu_seqlens[b+1]`` (int32).  ``prefix_k`` / ``prefix_v``: (P, kv_heads, head_dim), seen by every
-    query; they are read once for the whole batch.  ``k`` / ``v``: (rows, kv_heads, head_dim);
+    query, held once for the whole batch; for long prefixes of many short sequences their products run
+    over the stacked rows of the batch, otherwise every sequence goes through them.  ``k`` / ``v``: (rows, kv_heads, head_dim);
     sequence b owns rows ``kv_base[b] .. kv_base[b] + kv_lens[b]`` (int32, a cache stretch that ends
     with the keys of its queries), or, without both, the rows of its queries.  Key head j serves
     query heads ``j * heads / kv_heads ...``.  head_dim is 64 or 128; rows may be strided (column
@@ -284,10 +287,13 @@ def shared_prefix_attention(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, p
     queries are the last positions of their sequence).  ``scale`` (positive) defaults to
     head_dim ** -0.5.
 
-    Returns ``out`` (N, heads, head_dim); a query that sees no key gives zeros, rows of ``out``
-    behind ``cu_seqlens[-1]`` are not written.  Row numbers are checked on the device
-    (:func:`device_error` 611, 612).  The cut of the keys into parts depends on the batch, so a
-    sequence's result may differ in the last bits with its company; equal calls give equal bits."""
+    Returns ``out`` (N, heads, head_dim); a query that sees no key, or whose every score is -inf, gives
+    zeros, rows of ``out`` before ``cu_seqlens[0]`` and behind ``cu_seqlens[-1]`` are not written.  Row
+    numbers are checked on the device: :func:`device_error` 612 for own keys outside ``k`` (the
+    sequence is computed without own keys), 611 for ``cu_seqlens`` that decrease or leave 0 .. N (rows
+    next to such an entry hold nothing of use); nothing outside the tensors is touched.  The cut of the
+    keys into parts depends on the batch, so a sequence's result may differ in the last bits with its
+    company; equal calls give equal bits.  Forward only: the output carries no gradient."""
     if q.dim() != 3 or prefix_k.dim() != 3:
         raise ValueError("q must be (N, heads, head_dim), prefix_k (P, kv_heads, head_dim)")
     N, H, D = q.shape

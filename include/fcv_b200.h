@@ -419,10 +419,10 @@ int fcv_pack_rows(const void* src, int src_dtype, long batch_stride, int T, cons
  * Queries go to q_out (N rows), keys to k_out and, when v_out is given, the values unchanged to
  * v_out; kv_rows (int32, N) names the row of k_out / v_out for every token, a negative entry
  * stores nothing, rows must differ; null: token n goes to row n.  kv_limit = rows of k_out / v_out.
- * Outputs may be the inputs' own rows (in place).  A position outside the tables leaves the token
+ * Outputs may be the inputs' own rows (in place; with kv_rows only the queries).  A position outside the tables leaves the token
  * unwritten with device error 601, a row >= kv_limit its keys and values with 602.
  * head_dim 32, 64, 128 or 256; rope_half a multiple of 8; all rows, weights and tables 16-byte
- * aligned. */
+ * aligned (the stride of a single row is not used). */
 typedef struct fcv_qk_norm {
   const void* qkv;
   const float* q_weight;
@@ -451,10 +451,14 @@ int fcv_qk_norm_rope(const fcv_qk_norm* args, void* stream);
  *   q, out  (N, heads, head_dim) rows q_stride / out_stride elements apart
  *   k, v    (kv_rows, kv_heads, head_dim);  prefix_k, prefix_v (P, kv_heads, head_dim)
  * heads is a multiple of kv_heads (query head h reads key head h / (heads / kv_heads)); head_dim is
- * 64 or 128; scale is positive; rows 16-byte aligned.  Rows of out outside [cu_seqlens[0], cu_seqlens[B]) are left as
- * they were.  cu_seqlens that decrease or leave [0, N] give device error 611, own keys outside
- * [0, kv_rows) 612 (the sequence is computed without own keys).  Values must be finite where some
- * query of the same sequence sees them; rows behind a sequence's own keys may hold anything.
+ * 64 or 128; scale is positive and at most 2.3e38; rows 16-byte aligned (the stride of a single row is not
+ * used).  Rows of out outside [cu_seqlens[0], cu_seqlens[B]) are left as they were.  cu_seqlens that
+ * decrease or leave [0, N] give device error 611 (rows next to such an entry hold nothing of use), own keys
+ * outside [0, kv_rows) 612 (the sequence is computed without own keys; sequences without queries are
+ * checked too); nothing outside the tensors is touched.  A call with N = 0 or B = 0 launches nothing and
+ * checks no sequence.  Values must be finite where some
+ * query of the same sequence sees them; rows behind a sequence's own keys may hold anything.  A query
+ * whose every visible score is -inf gives zeros as well.
  * workspace: fcv_shared_prefix_workspace_bytes() bytes for the same arguments (0 for arguments that
  * are refused), 16-byte aligned; calls that may overlap need one each. */
 typedef struct fcv_prefix_attention {

@@ -763,3 +763,57 @@ def test_single_rows_of_odd_strides(dtype, P, H, Hkv):
     assert torch.equal(cache[:, Hkv * D:], qkv[:, (H + Hkv) * D:])
     q2, k2 = ops().qk_norm_rope(row, qw, kw, cos, sin, pos, H, Hkv, inplace=True)
     assert torch.equal(q2, q0) and torch.equal(k2, k0)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("way", list(WAYS))
+def test_first_offset_behind_the_first_row_and_a_stretch_of_keys_twice(way, dtype):
+    """Rows before the first sequence stay as they were, and two sequences may read one stretch of keys."""
+    args, q_lens, base, kv_lens = way_inputs(way, dtype)
+    used, P, D = sum(q_lens), args["prefix_k"].shape[0], args["q"].shape[2]
+    args["cu_seqlens"] += 3
+    base[-2], kv_lens[-2] = base[0], kv_lens[0]
+    t = lambda x: torch.tensor(x, dtype=torch.int32, device=DEV)  # noqa: E731
+    args["kv_base"], args["kv_lens"] = t(base), t(kv_lens)
+    out = torch.full(tuple(args["q"].shape), 7.0, dtype=dtype, device=DEV)
+    ops().shared_prefix_attention(**args, out=out)
+    assert (out[:3] == 7).all() and (out[3 + used:] == 7).all()
+    ref = attention_ref(args["q"][3:3 + used], args["k"], args["v"], args["prefix_k"], args["prefix_v"], q_lens, base,
+                        kv_lens, 1, D ** -0.5)
+    check_attention(out[3:3 + used], ref, P + max(kv_lens))
+
+
+@pytest.mark.parametrize("B,q_len,P,H,Hkv,D", [(700, 1, 3000, 16, 4, 64), (1500, 70, 50, 14, 2, 64),
+                                               (1300, 3, 20, 4, 2, 64)])
+def test_more_sequences_than_threads(B, q_len, P, H, Hkv, D):
+    """The kernels that go through the sequences with one block take several of them to a thread."""
+    rng = random.Random(B)
+    q_lens = [rng.randint(max(1, q_len // 2), q_len) for _ in range(B)]
+    past = [rng.randint(0, 90) for _ in range(B)]
+    run_case(q_lens, past, P, H, Hkv, D, torch.bfloat16, 1, 5)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("inter", [True, False])
+def test_norm_in_place_into_a_cache(dtype, inter):
+    """In place with a cache: the query columns are rewritten, keys and values go to the cache alone."""
+    n, H, Hkv, D = 70, 14, 2, 64
+    qkv, qw, kw, cos, sin, pos = norm_inputs(n, H, Hkv, D, 24, dtype, 15, pad=16)
+    keep = qkv.clone()
+    q0, k0 = ops().qk_norm_rope(qkv, qw, kw, cos, sin, pos, H, Hkv, interleaved=inter)
+    cache = torch.zeros(90, 2 * Hkv * D, dtype=dtype, device=DEV)
+    rows = torch.randperm(90, generator=gen(16), device=DEV)[:n].to(torch.int32)
+    q, same = ops().qk_norm_rope(qkv, qw, kw, cos, sin, pos, H, Hkv, interleaved=inter, inplace=True, kv_cache=cache,
+                                 kv_rows=rows)
+    assert same is cache and q.data_ptr() == qkv.data_ptr() and torch.equal(q, q0)
+    assert torch.equal(qkv[:, H * D:], keep[:, H * D:])
+    assert torch.equal(cache[rows.long()], torch.cat((k0.flatten(1), keep[:, (H + Hkv) * D:]), 1))
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("way", list(WAYS))
+def test_rows_whose_every_score_is_minus_infinity_are_zero(way, dtype):
+    args, q_lens, base, kv_lens = way_inputs(way, dtype, extra=0)
+    args["q"][..., 5] = args["q"][..., 5].abs() + 1
+    args["k"][..., 5] = args["prefix_k"][..., 5] = float("-inf")
+    assert (ops().shared_prefix_attention(**args) == 0).all()
