@@ -526,11 +526,16 @@ struct SpPlan {
 };
 // The estimates below choose between the ways of cutting.  They are fits, in microseconds on a B200, to
 // 356 shapes (1 to 128 sequences of 1 to 200 queries, prefixes of 200 to 8000 keys, 60 to 1200 own keys,
-// heads 16/16 and 14/2 of 64, 32/8 and 8/1 of 128) timed each way; the way that they choose is on
-// average 2 % slower than the best of the three.  Examples, tensor-core whole / whole / parts: one query
+// heads 16/16 and 14/2 of 64, 32/8 and 8/1 of 128, causal) timed each way; the way that they choose is on
+// average 1.5 % slower than the best of the three, by more than 20 % in 9 of them, at worst 1.84 times (4
+// sequences of about 160 queries behind 200 keys, up to 1200 own keys, 8/1 heads of 128: 69 us whole, 38 in
+// parts).  Examples, tensor-core whole / whole / parts: one query
 // of each of 4 streams behind 200 keys (16/16 heads) 13.4 / 7.4 / 15.7; behind 8000 keys 112 / 60 / 29;
 // 32 sequences of about 170 queries behind 2000 keys (32/8 heads) 256 / 688 / 396.
-// The own keys' lengths are on the device: a cache is taken to be half full.
+// The own keys' lengths are on the device: a cache is taken to be half full, up to 2048 keys a sequence.
+// A cache that is allotted far ahead of its content moves the choice: with 4096 rows to a sequence for the
+// same contents it is 2.3 % slower than the best on average, by more than 20 % in 17 shapes, at worst 2.06
+// times (32 one-query sequences behind 200 keys, up to 60 own keys, 8/1 heads of 128: 22 us against 11).
 SpPlan sp_plan(const fcv_prefix_attention& g) {
   const long N = g.N, P = g.P, kv_rows = g.kv_rows;
   const int B = g.B, H = g.heads, Hkv = g.kv_heads, D = g.head_dim;
@@ -1439,7 +1444,10 @@ int fcv_shared_prefix_attention(const fcv_prefix_attention* g, void* workspace, 
     }
     // A short prefix is given the few SMs on which it takes no longer than the own keys could (by the
     // rows of k, at most 30 us): the device's choice costs 3 us (64 streams behind 4096 keys: 46.5 us
-    // against 43.6), and being wrong costs little.
+    // against 43.6).  Over 20 shapes (64 to 200 streams behind 2000 to 4096 keys, caches filled from a
+    // thirtieth to full) the two take the same on average; short contents lose up to 1.18 times (64 streams of
+    // at most 60 own keys behind 3000, 32/8 heads of 128: 36.6 us against 31), full ones gain as much (128
+    // streams of 512 to 1024 behind 2000: 85 against 98).
     const float units = (float)kv_rows * kv_heads / kSpKeys + (float)B * kv_heads * (kSsItem + 1);
     const float most = std::min(30.f, std::max(12.f, 8.f + units * a.split.floor_us));
     for (int i = 0; i < a.split.n; ++i) {

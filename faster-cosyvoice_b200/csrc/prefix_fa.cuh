@@ -19,12 +19,18 @@
 // 64 x 16 MMA of S, at D = 128 64 clocks per 128 x 128 x 16 MMA of P V).  Neither bounds it: at D = 128
 // with two query tiles a step takes 2290 clocks, of which the MMAs fill 1280, and dropping the
 // exponentials, the MMAs, or both in a test build leaves 98, 89 and 62 % of the time -- the hand-overs
-// between softmax, issuer and tensor core (commit, mbarrier, wake-up) do.  Tensor memory allows no more
-// steps in flight: O takes 128 columns for each query tile.  Measured: 16 sequences of 700 to 1024
-// tokens behind 4096 keys, 32/8 heads of 128, 980 GFLOP: 990 us at burst clocks, 1110 us in a long run
-// (0.59 and 0.52 of the measured bf16 rates' burst figure, 0.64 of the sustained one).  Two threads to
-// a row (32 keys each, twice the warps) 1075 us; two S buffers with P over S, so that S of the next
-// tile and the store of P wait for nothing, 1000 us; both 1098 us.
+// between softmax, issuer and tensor core (commit, mbarrier, wake-up) do, once per 64 keys.  With P beside
+// S and O of 128 columns for each query tile, tensor memory holds one such step of two query tiles; steps
+// of 128 keys with P over S (2 x 128 + 2 x 128 columns) would halve the hand-overs and have not been built.
+// Measured: 16 sequences of 700 to 1024 tokens behind 4096 keys, 32/8 heads of 128, 980 GFLOP: 1115 us in
+// calls one after another, at power-capped clocks (0.52 of the measured bf16 burst rate, 0.64 of the
+// sustained one); 990 us in a short run (0.59 of burst).  In short runs, two threads to a row (32 keys
+// each, twice the warps) 1075 us; two S buffers with P over S, so that S of the next tile and the store of
+// P wait for nothing, 1000 us; both 1098 us.
+//
+// Roundings, each within those of one bf16 output: P goes to bf16 for its product (at most half a step,
+// 2^-8 relative, averaged over the keys) while its sum stays in float32; the polynomial share of the
+// exponentials is within 1.1e-4 (below 2^-12), the others are ex2.approx (2^-22).
 #pragma once
 
 #include "attn.cuh"

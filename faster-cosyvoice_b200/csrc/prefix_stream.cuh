@@ -295,6 +295,7 @@ __global__ void __launch_bounds__(SpStream<D>::THREADS, 1)
 #pragma unroll
           for (int d = 0; d < D / 8; ++d) o[d][0] *= e0, o[d][1] *= e0, o[d][2] *= e1, o[d][3] *= e1;
         }
+        // P is rounded to bf16 for the product (at most 2^-8 relative, averaged over the keys), its sum is not
         const uint32_t pf[4] = {pack_bf16x2(s[0][0], s[0][1]), pack_bf16x2(s[0][2], s[0][3]),
                                 pack_bf16x2(s[1][0], s[1][1]), pack_bf16x2(s[1][2], s[1][3])};
         // rows behind the sequence may hold anything, and a weight of zero does not stop a NaN
