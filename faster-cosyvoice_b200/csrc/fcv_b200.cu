@@ -667,8 +667,8 @@ SpPlan sp_plan(const fcv_prefix_attention& g) {
   } else if (p.fa_prefix && none) {
     // Even waves of parts, with the join's traffic; a ninth of the SMs is left to the join of the call
     // before (16 streams of 32/8 heads of 128 behind 16000 keys, calls one after another: 31 us in 128
-    // items, 35 in 144).  Chosen as beside own keys, or on the SMs left beside them, 14 shapes took 0.95 to
-    // 1.33 times as long (256 streams behind 8000 keys, 32/8 heads of 128: 65 us against 55).
+    // items, 35 in 144).  With room kept for own keys, 74 shapes took 0.95 to 3.2 times as long (256 streams
+    // behind 8000 keys, 32/8 heads of 128: 65 us against 55; 128 behind 200, 16/16 of 64: 37 against 11).
     p.fa_ctas = (int)sms;
     double best = 0;
     for (long n = 1; n <= 24 && (n == 1 || (n - 1) * 4 < tiles); ++n) {
@@ -823,7 +823,11 @@ int run_sp(const SpArgs& a, const SpPlan& p, cudaStream_t s) {
   }
   if (!a.whole) {
     const long warps = (long)a.N * a.H;
-    FCV_LAUNCH("sp_join_kernel", sp_join_kernel<T, D>, dim3((unsigned)((warps + 7) / 8)), dim3(256), 0, s, a);
+    const dim3 grid((unsigned)((warps + 7) / 8));
+    if (a.cuts == 0 && a.own_parts == 0)
+      FCV_LAUNCH("sp_join_kernel", sp_join_kernel<T, D, true>, grid, dim3(256), 0, s, a);
+    else
+      FCV_LAUNCH("sp_join_kernel", sp_join_kernel<T, D, false>, grid, dim3(256), 0, s, a);
   }
   return FCV_OK;
 }

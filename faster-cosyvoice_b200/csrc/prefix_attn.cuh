@@ -707,7 +707,9 @@ __device__ __forceinline__ int sp_pick_cuts(const SpSplit& s, int i) {
 // Joins the parts of a row: one warp per (token, head).  Its loads are a chain of round trips (the
 // token's sequence, the parts' maxima and sums, their outputs), so what can be read at once is: part by
 // part it took 24 us for 2048 rows of 17 parts, like this 7 us for the 5 parts that they have now.
-template <typename T, int D>
+// REPORT: without own parts no kernel before this one has looked at the sequences, so the first block
+// reports those out of range (behind a runtime check it cost every call 0.3 us).
+template <typename T, int D, bool REPORT>
 __global__ void __launch_bounds__(256) sp_join_kernel(const SpArgs a) {
   const int lane = threadIdx.x & 31;
   const long w = (long)blockIdx.x * 8 + (threadIdx.x >> 5);
@@ -736,8 +738,7 @@ __global__ void __launch_bounds__(256) sp_join_kernel(const SpArgs a) {
   }
   griddep_wait();
   griddep_launch();
-  // without own parts no kernel before this one has looked at the sequences
-  if (blockIdx.x == 0 && a.cuts == 0 && a.own_parts == 0)
+  if (REPORT && blockIdx.x == 0)
     for (int i = threadIdx.x; i < a.B; i += blockDim.x) sp_sequence(a, i, true);
   if (token >= a.N || token < begin || token >= end) return;  // rows behind the last sequence stay
   // own parts: all of them, or (cuts) one in the row's own place or one in each stretch that the item meets

@@ -102,13 +102,20 @@ __global__ void __launch_bounds__(1024) sp_list_kernel(const SpArgs a, int block
   __shared__ int hist[1024], most, total;
   __shared__ int2 lens[1024];  // queries and own keys of the first sequences; later ones are read each time
   const int tid = threadIdx.x, warp = tid >> 5, lane = tid & 31;
-  auto read = [&](int b, bool report) -> int2 {  // reports sequences without queries as well
-    const SpSeq s = sp_sequence(a, b, report);
-    return make_int2(s.nq, s.nk);
+  auto read = [&](int b, bool report) -> int2 {
+    const int c0 = a.cu[b], c1 = a.cu[b + 1];
+    int nq = c1 - c0;
+    const int nk = a.kv_lens ? a.kv_lens[b] : nq;
+    if (c0 < 0 || c1 < c0 || c1 > a.N) {
+      if (report) record_error(611);
+      nq = 0;
+    }
+    return make_int2(nq, nk);
   };
   for (int b = tid; b < a.B; b += 1024) {
     const int2 s = read(b, true);
     if (b < 1024) lens[b] = s;
+    if (s.x == 0) sp_sequence(a, b, true);  // without queries: no item will check its own keys
   }
   hist[tid] = 0;
   if (tid == 0) most = 1;
@@ -264,7 +271,20 @@ __global__ void __launch_bounds__(SpFa<D>::THREADS, 1)
         if (f.list) {
           o.hk = it % A.Hkv;
           const int2 e = f.list[it / A.Hkv];
-          const SpSeq s = sp_sequence(A, e.x, false);  // sp_list_kernel has reported it
+          SpSeq s;
+          {  // as sp_sequence(), by one thread
+            const int c0 = A.cu[e.x], c1 = A.cu[e.x + 1];
+            s.q0 = c0;
+            s.nq = c1 - c0;
+            if (c0 < 0 || c1 < c0 || c1 > A.N) s.q0 = s.nq = 0;
+            s.base = A.kv_base ? A.kv_base[e.x] : s.q0;
+            s.nk = A.kv_lens ? A.kv_lens[e.x] : s.nq;
+            if (s.nk < 0 || s.base < 0 || s.base + s.nk > A.kv_rows) {
+              if (s.nk != 0) record_error(612);
+              s.base = 0;
+              s.nk = 0;
+            }
+          }
           const int i0 = e.y * block;
           if (i0 >= s.nq) return false;
           o.tok0 = s.q0 + i0;
