@@ -628,7 +628,7 @@ def test_two_calls_at_once_on_two_streams():
     assert all(torch.equal(x, y) for x, y in got)
 
 
-@pytest.mark.parametrize("H,Hkv,D,P", [(32, 8, 128, 8000), (32, 8, 128, 3000), (16, 4, 64, 6000)])
+@pytest.mark.parametrize("H,Hkv,D,P", [(32, 8, 128, 8000), (32, 8, 128, 3000), (16, 4, 64, 6000), (20, 1, 128, 9000)])
 def test_no_own_keys_at_all_behind_a_long_prefix(H, Hkv, D, P):
     """Key tensors without rows leave the parts of the prefix alone; offsets and lengths that are out of
     range are still reported."""
